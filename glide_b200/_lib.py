@@ -101,6 +101,13 @@ SIGNATURES = {
     "glide_large_search_merged": (i32, [vp, vp, u32, vp, u32, P(SearchParamsC), vp, vp]),
     "glide_large_merged_graph": (i32, [vp, vp]),
     "glide_merge_results": (i32, [vp, vp, vp, u32, u32, u32, vp, vp]),
+    "glide_lookup_rows": (i32, [vp, vp, i32, u64, u32, u64, vp, u64, f32, vp, u64, vp]),
+    "glide_lookup_rows_grad_workspace": (C.c_size_t, [u64, u32, u64]),
+    "glide_lookup_rows_grad": (i32, [vp, vp, i32, u64, vp, u64, f32, vp, i32, u64, u32, u64, i32, vp, C.c_size_t, vp]),
+    "glide_dispatch_rows_workspace": (C.c_size_t, [u64, u32, u32]),
+    "glide_dispatch_rows": (i32, [vp, vp, i32, u64, u32, u64, vp, u32, u32, vp, u64, vp, vp, vp, vp, C.c_size_t, vp]),
+    "glide_combine_rows": (i32, [vp, vp, i32, u64, u32, u64, vp, u64, u32, vp, vp, u64, vp]),
+    "glide_combine_rows_grad": (i32, [vp, vp, i32, u64, u32, u64, vp, u64, u64, vp, u32, vp, vp, u64, vp, vp]),
     "glide_malloc": (i32, [vp, C.c_size_t, P(vp)]),
     "glide_memcpy_h2d": (i32, [vp, vp, vp, C.c_size_t]),
     "glide_memcpy_d2h": (i32, [vp, vp, vp, C.c_size_t]),

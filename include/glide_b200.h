@@ -408,6 +408,50 @@ void glide_large_last_stats(const glide_large *index, double out[8]);
 int glide_merge_results(glide_ctx *ctx, const uint32_t *d_ids, const float *d_dists, uint32_t sets, uint32_t q,
                         uint32_t top_k, uint32_t *d_out_ids, float *d_out_dists);
 
+/* ---- rows by ids and by partitions ------------------------------------------------------- */
+/* Operators on the rows of a table, for hosts that train or serve what an index is built over; the reference has none.
+ * They differ from the calls above in four ways: they enqueue on `stream` (a cudaStream_t of the context's device; NULL is
+ * the default stream) and return without waiting, so that they can be captured into a graph; they take their scratch
+ * from the caller (at least as many bytes as the _workspace function says, aligned to 256 bytes, one workspace for each
+ * call that may run at the same time); the calling thread's current device stays as it was; rows are of any of the types below, `stride`
+ * counts the values from one row to the next (inputs: any stride, 0 repeats a row; results: at least dim). Results may not
+ * overlap other arguments. Sums are fp32 in an order that the arguments determine: equal calls give equal bits. */
+enum { GLIDE_ROW_F32 = 0, GLIDE_ROW_U8 = 1, GLIDE_ROW_F16 = 2, GLIDE_ROW_BF16 = 3 };
+/* d_out[t] = scale * d_table[d_ids[t]], rounded once; a row of zeros for ids of n and beyond, such as the 0xffffffff that a
+ * search leaves in an unfilled place. d_out has the table's type, fp32 for a table of bytes. */
+int glide_lookup_rows(glide_ctx *ctx, const void *d_table, int row_type, uint64_t n, uint32_t dim, uint64_t table_stride,
+                      const uint32_t *d_ids, uint64_t count, float scale, void *d_out, uint64_t out_stride, void *stream);
+/* The gradient of glide_lookup_rows with respect to the table: d_table_grad[v] = scale * the sum of d_grad[t] over all t with
+ * d_ids[t] == v, zeros where there is none; with accumulate != 0 the sum is added to what d_table_grad holds and the
+ * other rows stay as they are. d_table_grad has the type of d_grad or fp32. */
+size_t glide_lookup_rows_grad_workspace(uint64_t n, uint32_t dim, uint64_t count);
+int glide_lookup_rows_grad(glide_ctx *ctx, const void *d_grad, int row_type, uint64_t grad_stride, const uint32_t *d_ids, uint64_t count,
+                           float scale, void *d_table_grad, int grad_type, uint64_t n, uint32_t dim, uint64_t table_grad_stride,
+                           int accumulate, void *d_workspace, size_t workspace_bytes, void *stream);
+/* Rows sorted by the partitions (experts) that they chose. d_choice: count x choices, a partition or anything from `partitions`
+ * on (0xffffffff) for no choice. The pairs (t, j) with a choice, sorted by (choice, t, j), are places 0, 1, ...:
+ * d_sorted[p] = d_rows[t], d_map[p] = t, d_position[t * choices + j] = p. d_segment_start[s] is the first place of
+ * partition s, d_segment_start[partitions] the number of places taken. d_sorted and d_map have count * choices rows; those behind
+ * the last place taken are left as they were in d_sorted and are 0xffffffff in d_map, as is d_position of a pair without a choice.
+ * choices <= 128, partitions <= 4096. The gradient with respect to d_rows is glide_combine_rows without weights. */
+size_t glide_dispatch_rows_workspace(uint64_t count, uint32_t choices, uint32_t partitions);
+int glide_dispatch_rows(glide_ctx *ctx, const void *d_rows, int row_type, uint64_t count, uint32_t dim, uint64_t row_stride,
+                        const uint32_t *d_choice, uint32_t choices, uint32_t partitions, void *d_sorted, uint64_t sorted_stride,
+                        uint32_t *d_position, uint32_t *d_map, uint32_t *d_segment_start, void *d_workspace, size_t workspace_bytes,
+                        void *stream);
+/* d_out[t] = the sum over j, in order, of weight[t, j] * d_sorted[d_position[t, j]] (null weights: 1), rounded once; pairs
+ * whose position is sorted_rows or beyond are left out, whatever their weight. */
+int glide_combine_rows(glide_ctx *ctx, const void *d_sorted, int row_type, uint64_t sorted_rows, uint32_t dim, uint64_t sorted_stride,
+                       const uint32_t *d_position, uint64_t count, uint32_t choices, const float *d_weights_or_null, void *d_out,
+                       uint64_t out_stride, void *stream);
+/* The gradients of glide_combine_rows: d_grad_sorted[d_position[t, j]] = weight[t, j] * d_grad[t] (rows that no position names
+ * are left as they were; a position that occurs twice is written twice, in any order), d_grad_weights[t, j] =
+ * <d_grad[t], d_sorted[d_position[t, j]]>, 0 for a pair that was left out. */
+int glide_combine_rows_grad(glide_ctx *ctx, const void *d_grad, int row_type, uint64_t count, uint32_t dim, uint64_t grad_stride,
+                            const void *d_sorted, uint64_t sorted_rows, uint64_t sorted_stride, const uint32_t *d_position,
+                            uint32_t choices, const float *d_weights_or_null, void *d_grad_sorted, uint64_t grad_sorted_stride,
+                            float *d_grad_weights_or_null, void *stream);
+
 /* ---- device memory helpers for hosts without their own CUDA binding --------------------- */
 int glide_malloc(glide_ctx *ctx, size_t bytes, void **d_out);
 int glide_memcpy_h2d(glide_ctx *ctx, void *d_dst, const void *h_src, size_t bytes);
