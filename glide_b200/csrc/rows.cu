@@ -24,9 +24,10 @@ constexpr uint32_t kNone = 0xffffffffu;
 constexpr uint32_t kMaxPartitions = 4096;   // of dispatch_rows: a counter for each and warp in shared memory
 constexpr uint32_t kMaxChoices = 128;       // as many as glide_bruteforce_knn returns neighbours
 constexpr uint32_t kMaxDim = 1u << 20;
-constexpr uint32_t kTile = 2048;            // items of a CTA in the counting sort
-constexpr uint32_t kSortThreads = 256, kSortWarps = kSortThreads / 32, kWarpItems = kTile / kSortWarps;
-constexpr uint32_t kChunk = 32;             // sorted items that one group of lanes joins in the gradient
+constexpr uint32_t kRounds = 8;             // items of a thread in the counting sort
+constexpr uint32_t kMaxPassBits = 11;       // digits of a pass: 32 warps' counters take 128 KB of shared memory
+constexpr uint32_t kMaxFusedTiles = 64;     // tiles whose counts every CTA of the second kernel adds up by itself
+constexpr uint32_t kSmallPairs = 2048;      // pairs that dispatch_rows places and copies in one launch
 
 // ---- rows as words ----------------------------------------------------------------------------------------
 template<int B> struct Word;
@@ -46,6 +47,25 @@ template<> __device__ __forceinline__ float from_float<float>(float x) { return 
 template<> __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
 template<> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
+// A word from or to global memory as ONE access: a plain dereference that is copied into values of T next is split into
+// accesses of T by the compiler (93 % L1 hits and a quarter of the bandwidth in combine_kernel).
+template<bool kWritten, typename W>
+__device__ __forceinline__ W get_word(const W *p) {
+    if constexpr (kWritten) return __ldcg(p);
+    else return __ldg(p);
+}
+// Zeros where the word is not wanted. The words of several rows are fetched before any of them is taken apart: with the
+// conversion inside the condition each load is waited for before the next (1.9 of 6.5 TB/s in combine_kernel).
+template<typename W, typename T>
+__device__ __forceinline__ W get_word_if(const T *p, bool wanted) {
+    W w;
+    memset(&w, 0, sizeof w);
+    if (wanted) w = __ldg(reinterpret_cast<const W *>(p));
+    return w;
+}
+template<typename W>
+__device__ __forceinline__ void put_word(W *p, const W &w) { __stcg(p, w); }
+
 template<typename T, int V>
 __device__ __forceinline__ void unpack(const WordOf<T, V> &w, float (&f)[V]) {
     T t[V];
@@ -63,7 +83,7 @@ __device__ __forceinline__ void store(T *p, const float (&f)[V]) {
         for (int i = 0; i < V; i++) t[i] = from_float<T>(f[i]);
         WordOf<T, V> w;
         memcpy(&w, t, sizeof w);
-        *reinterpret_cast<WordOf<T, V> *>(p) = w;
+        put_word(reinterpret_cast<WordOf<T, V> *>(p), w);
     } else {
         constexpr int H = 16 / (int) sizeof(T);
 #pragma unroll
@@ -76,16 +96,17 @@ __device__ __forceinline__ void store(T *p, const float (&f)[V]) {
     }
 }
 
-template<typename T, int V>
+// kWritten: the memory is written in the same launch (each word by the thread that reads it)
+template<typename T, int V, bool kWritten = false>
 __device__ __forceinline__ void load(const T *p, float (&f)[V]) {
     if constexpr (sizeof(T) * V <= 16) {
-        unpack<T, V>(*reinterpret_cast<const WordOf<T, V> *>(p), f);
+        unpack<T, V>(get_word<kWritten>(reinterpret_cast<const WordOf<T, V> *>(p)), f);
     } else {
         constexpr int H = 16 / (int) sizeof(T);
 #pragma unroll
         for (int h = 0; h < V / H; h++) {
             float g[H];
-            load<T, H>(p + h * H, g);
+            load<T, H, kWritten>(p + h * H, g);
 #pragma unroll
             for (int i = 0; i < H; i++) f[h * H + i] = g[i];
         }
@@ -119,53 +140,74 @@ __global__ void __launch_bounds__(256) lookup_kernel(const T *__restrict__ table
         at[u] = (x - row[u] * words.d) * V;
         id[u] = ids[row[u]];
     }
-    float f[U][V];
+    WordOf<T, V> w[U];
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-        if (id[u] < n) {
-            load<T, V>(table + (uint64_t) id[u] * table_stride + at[u], f[u]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < V; i++) f[u][i] = 0.0f;
-        }
-    }
+    for (int u = 0; u < U; u++) w[u] = get_word_if<WordOf<T, V>>(table + (uint64_t) id[u] * table_stride + at[u], id[u] < n);
 #pragma unroll
     for (int u = 0; u < U; u++) {
         if (first + u * 256 >= units) break;
+        float f[V];
+        unpack<T, V>(w[u], f);
 #pragma unroll
-        for (int i = 0; i < V; i++) f[u][i] = id[u] < n ? f[u][i] * scale : 0.0f;
-        store<O, V>(out + (uint64_t) row[u] * out_stride + at[u], f[u]);
+        for (int i = 0; i < V; i++) f[i] = id[u] < n ? f[i] * scale : 0.0f;
+        store<O, V>(out + (uint64_t) row[u] * out_stride + at[u], f);
     }
+}
+
+// ---- launches that follow one another -----------------------------------------------------------------------------
+// The kernels of one call are launched as programmatic dependents: the next one's CTAs become resident while the last one
+// drains, and wait() holds them until everything before is complete and visible.
+__device__ __forceinline__ void wait_for_previous() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+template<typename... P, typename... A>
+cudaError_t launch(void (*kernel)(P...), uint64_t grid, uint32_t block, uint32_t smem, cudaStream_t stream, bool dependent, A... args) {
+    if (smem > 48 * 1024) {   // more dynamic shared memory than a kernel gets unasked
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem);
+        if (e != cudaSuccess) return e;
+    }
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3((uint32_t) grid);
+    config.blockDim = dim3(block);
+    config.dynamicSmemBytes = smem;
+    config.stream = stream;
+    config.attrs = &attr;
+    config.numAttrs = dependent ? 1 : 0;
+    return cudaLaunchKernelEx(&config, kernel, static_cast<P>(args)...);
 }
 
 // ---- stable counting sort -------------------------------------------------------------------------------------
 // One pass places every item behind all items of a smaller digit and behind the items of its own digit that came before it.
-// count: a CTA takes kTile consecutive items, each of its warps a run of them 32 at a time; a lane's rank among the items of
+// A CTA takes a tile of consecutive items, each of its warps a run of 256, 32 at a time: a lane's rank among the items of
 // its digit is the warp's running count plus the equal digits at lower lanes, and a scan over the warps' counts makes it the
-// rank in the CTA. scan: the counts of all CTAs become, digit by digit, counts of the CTAs before. No atomics: the order
-// depends on nothing but the keys.
+// rank in the tile. No atomics: the order depends on nothing but the keys. Few launches count most here (the data are 6 bytes
+// an item): one tile is sorted by one launch, up to kMaxFusedTiles by two launches a pass (every CTA of the second adds up
+// the counts of all tiles), more by three.
 struct Digit {
     uint32_t limit, shift, mask;   // keys beyond limit count as limit
     __device__ __forceinline__ uint32_t of(uint32_t key) const { return (min(key, limit) >> shift) & mask; }
 };
 
-__global__ void __launch_bounds__(kSortThreads) bucket_count_kernel(const uint32_t *__restrict__ keys, uint32_t items, Digit digit,
-                                                                    uint32_t buckets, uint32_t *__restrict__ counts,
-                                                                    uint16_t *__restrict__ ranks) {
-    extern __shared__ uint16_t warp_counts[];   // kSortWarps x buckets
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-    for (uint32_t i = threadIdx.x; i < kSortWarps * buckets; i += kSortThreads) warp_counts[i] = 0;
+__device__ __forceinline__ uint32_t warp_items() { return kRounds * 32; }
+__device__ __forceinline__ uint32_t tile_item(uint32_t r) {   // of this thread, from the tile's first
+    return (threadIdx.x >> 5) * warp_items() + r * 32 + (threadIdx.x & 31u);
+}
+
+// Ranks in the tile of this thread's items by their digits (kNone: no item), and the tile's count of each bucket through `put`.
+template<typename Put>
+__device__ __forceinline__ void rank_tile(const uint32_t (&d)[kRounds], uint32_t buckets, uint16_t *warp_counts, uint32_t (&rank)[kRounds], Put put) {
+    const uint32_t warps = blockDim.x >> 5, lane = threadIdx.x & 31u;
+    const uint32_t words = (warps * buckets + 7) / 8;
+    for (uint32_t i = threadIdx.x; i < words; i += blockDim.x) reinterpret_cast<uint4 *>(warp_counts)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
-    uint16_t *mine = warp_counts + warp * buckets;
-    const uint32_t first = blockIdx.x * kTile + warp * kWarpItems;
-    uint32_t d[kWarpItems / 32], rank[kWarpItems / 32];
+    uint16_t *mine = warp_counts + (threadIdx.x >> 5) * buckets;
 #pragma unroll
-    for (uint32_t r = 0; r < kWarpItems / 32; r++) {
-        const uint32_t i = first + r * 32 + lane;
-        d[r] = i < items ? digit.of(keys[i]) : kNone;
-    }
-#pragma unroll
-    for (uint32_t r = 0; r < kWarpItems / 32; r++) {
+    for (uint32_t r = 0; r < kRounds; r++) {
         const uint32_t same = __match_any_sync(0xffffffffu, d[r]);
         const bool there = d[r] != kNone;
         const uint32_t before = there ? mine[d[r]] : 0;
@@ -175,27 +217,108 @@ __global__ void __launch_bounds__(kSortThreads) bucket_count_kernel(const uint32
         __syncwarp();
     }
     __syncthreads();
-    for (uint32_t b = threadIdx.x; b < buckets; b += kSortThreads) {
+    for (uint32_t b = threadIdx.x; b < buckets; b += blockDim.x) {
         uint32_t sum = 0;
-#pragma unroll
-        for (uint32_t w = 0; w < kSortWarps; w++) {
+        for (uint32_t w = 0; w < warps; w++) {
             const uint32_t c = warp_counts[w * buckets + b];
             warp_counts[w * buckets + b] = (uint16_t) sum;
             sum += c;
         }
-        counts[(uint64_t) blockIdx.x * buckets + b] = sum;
+        put(b, sum);
     }
     __syncthreads();
 #pragma unroll
-    for (uint32_t r = 0; r < kWarpItems / 32; r++) {
-        const uint32_t i = first + r * 32 + lane;
-        if (i < items) ranks[i] = (uint16_t) (mine[d[r]] + rank[r]);
+    for (uint32_t r = 0; r < kRounds; r++)
+        if (d[r] != kNone) rank[r] += mine[d[r]];
+}
+
+__host__ __device__ constexpr uint32_t rank_smem(uint32_t warps, uint32_t buckets) { return (warps * buckets + 7) / 8 * 16; }
+
+// Exclusive sums over `buckets` values, in place in shared memory, which the CTA has written.
+__device__ __forceinline__ void scan_buckets(uint32_t *values, uint32_t buckets) {
+    __shared__ uint32_t warp_sum[32];
+    __shared__ uint32_t all;
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    uint32_t carry = 0;
+    for (uint32_t b0 = 0; b0 < buckets; b0 += blockDim.x) {
+        __syncthreads();
+        const uint32_t b = b0 + threadIdx.x, v = b < buckets ? values[b] : 0;
+        uint32_t incl = v;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const uint32_t o = __shfl_up_sync(0xffffffffu, incl, off);
+            if (lane >= (uint32_t) off) incl += o;
+        }
+        if (lane == 31) warp_sum[warp] = incl;
+        __syncthreads();
+        if (warp == 0) {
+            uint32_t w = lane < warps ? warp_sum[lane] : 0, sum = w;
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+                const uint32_t o = __shfl_up_sync(0xffffffffu, sum, off);
+                if (lane >= (uint32_t) off) sum += o;
+            }
+            warp_sum[lane] = sum - w;
+            if (lane == 31) all = sum;
+        }
+        __syncthreads();
+        if (b < buckets) values[b] = carry + warp_sum[warp] + incl - v;
+        carry += all;
+    }
+    __syncthreads();
+}
+
+// Where a pass leaves its items. Radix: keys and values in their new order; values_in == nullptr: an item's value is its index.
+struct ToSorted {
+    const uint32_t *values_in;
+    uint32_t *keys, *values;
+    __device__ __forceinline__ uint32_t value_of(uint32_t i) const { return values_in ? values_in[i] : i; }
+    __device__ __forceinline__ void item(uint32_t, uint32_t value, uint32_t key, const Digit &, uint32_t place) const {
+        keys[place] = key;
+        values[place] = value;
+    }
+    __device__ __forceinline__ void start(uint32_t, uint32_t) const {}
+};
+
+// Dispatch: the place of every pair, the row at every place, the first place of every partition. Pairs without a partition are
+// the last bucket, so that the tail of the map is theirs.
+struct ToPlaces {
+    uint32_t *position, *map, *segment_start;
+    Div choices;
+    __device__ __forceinline__ uint32_t value_of(uint32_t i) const { return i; }
+    __device__ __forceinline__ void item(uint32_t pair, uint32_t, uint32_t key, const Digit &digit, uint32_t place) const {
+        const bool there = key < digit.limit;
+        position[pair] = there ? place : kNone;
+        map[place] = there ? choices.of(pair) : kNone;
+    }
+    __device__ __forceinline__ void start(uint32_t bucket, uint32_t place) const { segment_start[bucket] = place; }
+};
+
+__global__ void __launch_bounds__(1024) bucket_count_kernel(const uint32_t *__restrict__ keys, uint32_t items, Digit digit, uint32_t buckets,
+                                                            uint32_t *__restrict__ counts, uint16_t *__restrict__ ranks) {
+    extern __shared__ __align__(16) uint16_t warp_counts[];
+    wait_for_previous();
+    const uint32_t first = blockIdx.x * (blockDim.x * kRounds);
+    uint32_t d[kRounds], rank[kRounds];
+#pragma unroll
+    for (uint32_t r = 0; r < kRounds; r++) {
+        const uint32_t i = first + tile_item(r);
+        d[r] = i < items ? digit.of(keys[i]) : kNone;
+    }
+    uint32_t *mine = counts + (uint64_t) blockIdx.x * buckets;
+    rank_tile(d, buckets, warp_counts, rank, [&](uint32_t b, uint32_t sum) { mine[b] = sum; });
+#pragma unroll
+    for (uint32_t r = 0; r < kRounds; r++) {
+        const uint32_t i = first + tile_item(r);
+        if (i < items) ranks[i] = (uint16_t) rank[r];
     }
 }
 
+// The counts of all tiles become, bucket by bucket, counts of the tiles before, and totals.
 __global__ void __launch_bounds__(1024) bucket_scan_kernel(uint32_t *__restrict__ counts, uint32_t tiles, uint32_t buckets,
                                                            uint32_t *__restrict__ totals) {
     __shared__ uint32_t part[32][33];
+    wait_for_previous();
     const uint32_t x = threadIdx.x & 31u, y = threadIdx.x >> 5;
     const uint32_t b = blockIdx.x * 32 + x;
     const uint32_t each = (tiles + 31) / 32, t0 = min(y * each, tiles), t1 = min(t0 + each, tiles);
@@ -216,58 +339,113 @@ __global__ void __launch_bounds__(1024) bucket_scan_kernel(uint32_t *__restrict_
     }
 }
 
-// The first place of every bucket, from the buckets' totals, into shared memory; every thread of the CTA calls it.
-template<uint32_t kThreads>
-__device__ __forceinline__ void bucket_starts(const uint32_t *__restrict__ totals, uint32_t buckets, uint32_t *starts) {
-    __shared__ uint32_t warp_sum[kThreads / 32];
-    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
-    const uint32_t each = (buckets + kThreads - 1) / kThreads, b0 = min(threadIdx.x * each, buckets), b1 = min(b0 + each, buckets);
-    uint32_t sum = 0;
-    for (uint32_t b = b0; b < b1; b++) sum += totals[b];
-    uint32_t incl = sum;
+template<typename To, bool kScanned>
+__global__ void __launch_bounds__(1024) bucket_place_kernel(const uint32_t *__restrict__ keys, uint32_t items, Digit digit, uint32_t buckets,
+                                                            const uint32_t *__restrict__ counts, uint32_t tiles, const uint32_t *__restrict__ totals,
+                                                            const uint16_t *__restrict__ ranks, To to) {
+    extern __shared__ __align__(16) uint32_t base[];   // of each bucket: all items of smaller ones, then the tiles before, too
+    wait_for_previous();
+    const uint32_t first = blockIdx.x * (blockDim.x * kRounds);
+    uint32_t key[kRounds], rank[kRounds], value[kRounds];
 #pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-        const uint32_t o = __shfl_up_sync(0xffffffffu, incl, off);
-        if (lane >= (uint32_t) off) incl += o;
+    for (uint32_t r = 0; r < kRounds; r++) {
+        const uint32_t i = min(first + r * blockDim.x + threadIdx.x, items - 1);
+        key[r] = min(keys[i], digit.limit);
+        rank[r] = ranks[i];
+        value[r] = to.value_of(i);
     }
-    if (lane == 31) warp_sum[warp] = incl;
+    uint32_t before[(kMaxPartitions + 1 + 511) / 512];   // the launcher gives a thread no more buckets than that
+    uint32_t n = 0;
+#pragma unroll
+    for (uint32_t q = 0; q < sizeof before / sizeof *before; q++) {
+        const uint32_t b = q * blockDim.x + threadIdx.x;
+        if (b >= buckets) break;
+        uint32_t all = 0, mine = 0;
+        if constexpr (kScanned) {
+            all = totals[b];
+            mine = counts[(uint64_t) blockIdx.x * buckets + b];
+        } else {
+#pragma unroll 8
+            for (uint32_t t = 0; t < tiles; t++) {
+                const uint32_t c = counts[(uint64_t) t * buckets + b];
+                mine += t < blockIdx.x ? c : 0;
+                all += c;
+            }
+        }
+        base[b] = all;
+        before[q] = mine;
+        n = q + 1;
+    }
+    scan_buckets(base, buckets);
+#pragma unroll
+    for (uint32_t q = 0; q < sizeof before / sizeof *before; q++) {
+        if (q >= n) break;
+        const uint32_t b = q * blockDim.x + threadIdx.x;
+        if (blockIdx.x == 0) to.start(b, base[b]);
+        base[b] += before[q];
+    }
     __syncthreads();
-    uint32_t run = incl - sum;
-    for (uint32_t w = 0; w < warp; w++) run += warp_sum[w];
-    for (uint32_t b = b0; b < b1; b++) {
-        starts[b] = run;
-        run += totals[b];
+#pragma unroll
+    for (uint32_t r = 0; r < kRounds; r++) {
+        const uint32_t i = first + r * blockDim.x + threadIdx.x;
+        if (i < items) to.item(i, value[r], key[r], digit, base[digit.of(key[r])] + rank[r]);
+    }
+}
+
+// One tile: ranks and places in one launch.
+template<typename To>
+__device__ __forceinline__ void sort_tile(const uint32_t *keys, uint32_t items, const Digit &digit, uint32_t buckets, uint32_t *base, uint16_t *warp_counts, const To &to) {
+    uint32_t key[kRounds], d[kRounds], rank[kRounds], value[kRounds];
+#pragma unroll
+    for (uint32_t r = 0; r < kRounds; r++) {
+        const uint32_t i = tile_item(r);
+        key[r] = i < items ? min(keys[i], digit.limit) : kNone;
+        d[r] = i < items ? digit.of(key[r]) : kNone;
+        value[r] = i < items ? to.value_of(i) : 0;
+    }
+    rank_tile(d, buckets, warp_counts, rank, [&](uint32_t b, uint32_t sum) { base[b] = sum; });
+    scan_buckets(base, buckets);
+    for (uint32_t b = threadIdx.x; b < buckets; b += blockDim.x) to.start(b, base[b]);
+#pragma unroll
+    for (uint32_t r = 0; r < kRounds; r++) {
+        const uint32_t i = tile_item(r);
+        if (i < items) to.item(i, value[r], key[r], digit, base[d[r]] + rank[r]);
     }
     __syncthreads();
 }
 
-// The items of one pass in their new places. values == nullptr: an item's value is its index.
-__global__ void __launch_bounds__(kSortThreads) bucket_scatter_kernel(const uint32_t *__restrict__ keys, const uint32_t *__restrict__ values,
-                                                                      uint32_t items, Digit digit, uint32_t buckets,
-                                                                      const uint32_t *__restrict__ before, const uint32_t *__restrict__ totals,
-                                                                      const uint16_t *__restrict__ ranks, uint32_t *__restrict__ keys_out,
-                                                                      uint32_t *__restrict__ values_out) {
-    extern __shared__ uint32_t starts[];
-    bucket_starts<kSortThreads>(totals, buckets, starts);
-#pragma unroll
-    for (uint32_t r = 0; r < kTile / kSortThreads; r++) {
-        const uint32_t i = blockIdx.x * kTile + r * kSortThreads + threadIdx.x;
-        if (i >= items) break;
-        const uint32_t key = min(keys[i], digit.limit), d = digit.of(key);
-        const uint32_t p = starts[d] + before[(uint64_t) blockIdx.x * buckets + d] + ranks[i];
-        keys_out[p] = key;
-        values_out[p] = values ? values[i] : i;
+__global__ void __launch_bounds__(1024) place_tile_kernel(const uint32_t *keys, uint32_t items, Digit digit, uint32_t buckets, ToPlaces to) {
+    extern __shared__ __align__(16) uint16_t warp_counts[];
+    uint32_t *base = reinterpret_cast<uint32_t *>(reinterpret_cast<char *>(warp_counts) + rank_smem(blockDim.x >> 5, buckets));
+    wait_for_previous();
+    sort_tile(keys, items, digit, buckets, base, warp_counts, to);
+}
+
+// All passes of a radix sort of one tile; the items lie in global memory between passes (the CTA's barriers order them).
+__global__ void __launch_bounds__(1024) sort_tile_kernel(const uint32_t *keys, uint32_t items, uint32_t limit, uint32_t bits, uint32_t pass_bits,
+                                                         uint32_t *keys0, uint32_t *values0, uint32_t *keys1, uint32_t *values1) {
+    extern __shared__ __align__(16) uint16_t warp_counts[];
+    uint32_t *base = reinterpret_cast<uint32_t *>(reinterpret_cast<char *>(warp_counts) + rank_smem(blockDim.x >> 5, 1u << pass_bits));
+    wait_for_previous();
+    const uint32_t *in = keys, *values = nullptr;
+    for (uint32_t shift = 0, pass = 0; shift < bits; shift += pass_bits, pass++) {
+        uint32_t *k = pass & 1 ? keys1 : keys0, *v = pass & 1 ? values1 : values0;
+        const uint32_t here = min(pass_bits, bits - shift);
+        sort_tile(in, items, Digit{limit, shift, (1u << here) - 1}, 1u << here, base, warp_counts, ToSorted{values, k, v});
+        in = k;
+        values = v;
     }
 }
 
 // ---- gradient of a lookup ---------------------------------------------------------------------------------------
 struct GradArgs {
     const uint32_t *keys, *values;   // sorted by id: the id, and the row of grad_out
-    uint32_t items, n, dim, words, lanes, slabs;
+    uint32_t items, n, dim, words, lanes, slabs, chunk;
     float scale;
     uint64_t in_stride, out_stride;
     int accumulate;
     float *partial;                  // (2 * chunk + which) * dim: sums of runs that leave their chunk
+    uint32_t join_blocks, zero_rows; // CTAs that join; the others clear zero_rows rows each
 };
 
 template<typename O, int V>
@@ -277,23 +455,69 @@ __device__ __forceinline__ void put_grad(O *out, const GradArgs &a, uint32_t id,
     for (int i = 0; i < V; i++) acc[i] *= a.scale;
     if (a.accumulate) {
         float old[V];
-        load<O, V>(p, old);
+        load<O, V, true>(p, old);
 #pragma unroll
         for (int i = 0; i < V; i++) acc[i] += old[i];
     }
     store<O, V>(p, acc);
 }
 
-// A group of lanes joins kChunk sorted items over a slab of the row: the sum of a run of equal ids goes to the id's row, or,
+// The first of the sorted keys from `lo` on that is not below `key`; the CTA narrows the range by its width at each step.
+__device__ __forceinline__ uint32_t first_not_below(const uint32_t *__restrict__ keys, uint32_t lo, uint32_t hi, uint32_t key) {
+    while (lo < hi) {
+        const uint32_t step = (hi - lo + blockDim.x - 1) / blockDim.x;
+        const uint64_t i = lo + (uint64_t) threadIdx.x * step;
+        const uint32_t below = __syncthreads_count(i < hi && keys[i] < key);
+        if (below == 0) break;
+        const uint64_t end = lo + (uint64_t) below * step;
+        lo += (below - 1) * step + 1;
+        if (end < hi) hi = (uint32_t) end;
+    }
+    return lo;
+}
+
+// Rows [r0, r1) that no id names are cleared.
+template<typename O, int V>
+__device__ __forceinline__ void clear_rows(O *out, const GradArgs &a, uint32_t r0, uint32_t r1) {
+    __shared__ uint32_t named[256 / 32];   // a CTA clears 256 rows at most
+    if (threadIdx.x < 8) named[threadIdx.x] = 0;
+    __syncthreads();
+    uint32_t at = first_not_below(a.keys, 0, a.items, r0);
+    while (at < a.items) {
+        const uint32_t i = at + threadIdx.x, key = i < a.items ? a.keys[i] : kNone;
+        if (key < r1) atomicOr(&named[(key - r0) >> 5], 1u << ((key - r0) & 31u));
+        const uint32_t here = __syncthreads_count(key < r1);
+        if (here < blockDim.x) break;
+        // a whole CTA's width of one id: on to the next id
+        const uint32_t head = a.keys[at];
+        at = a.keys[at + blockDim.x - 1] == head ? first_not_below(a.keys, at + blockDim.x, a.items, head + 1) : at + blockDim.x;
+    }
+    __syncthreads();
+    float zero[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) zero[i] = 0.0f;
+    for (uint32_t x = threadIdx.x; x < (r1 - r0) * a.words; x += blockDim.x) {
+        const uint32_t r = x / a.words, w = x - r * a.words;
+        if (!(named[r >> 5] >> (r & 31u) & 1u)) store<O, V>(out + (uint64_t) (r0 + r) * a.out_stride + w * V, zero);
+    }
+}
+
+// A group of lanes joins a chunk of sorted items over a slab of the row: the sum of a run of equal ids goes to the id's row, or,
 // where the run goes on in another chunk, to the chunk's partial sums (first: it came from the chunk before).
 template<typename T, typename O, int V>
 __global__ void __launch_bounds__(256) grad_join_kernel(const T *__restrict__ grad, O *__restrict__ out, GradArgs a) {
     constexpr int U = 8;
+    wait_for_previous();
+    if (blockIdx.x >= a.join_blocks) {
+        const uint64_t r0 = (uint64_t) (blockIdx.x - a.join_blocks) * a.zero_rows;
+        clear_rows<O, V>(out, a, (uint32_t) r0, (uint32_t) min((uint64_t) a.n, r0 + a.zero_rows));
+        return;
+    }
     const uint32_t group = (blockIdx.x * 256 + threadIdx.x) / a.lanes, lane = threadIdx.x & (a.lanes - 1);
     const uint32_t chunk = group / a.slabs, word = (group - chunk * a.slabs) * a.lanes + lane;
-    const uint32_t c0 = chunk * kChunk;
+    const uint64_t c0 = (uint64_t) chunk * a.chunk;
     if (c0 >= a.items || word >= a.words) return;
-    const uint32_t c1 = min(c0 + kChunk, a.items), at = word * V;
+    const uint32_t c1 = (uint32_t) min(c0 + a.chunk, (uint64_t) a.items), at = word * V;
     uint32_t id = a.keys[c0];
     bool from_left = c0 > 0 && a.keys[c0 - 1] == id;
     float acc[V];
@@ -301,18 +525,20 @@ __global__ void __launch_bounds__(256) grad_join_kernel(const T *__restrict__ gr
     for (int i = 0; i < V; i++) acc[i] = 0.0f;
     auto put = [&](bool to_right) {
         if (id >= a.n) return;
-        if (from_left || to_right) store<float, V>(a.partial + (uint64_t) (2 * chunk + (from_left ? 0 : 1)) * a.dim + at, acc);
+        if (from_left || to_right) store<float, V>(a.partial + (2ull * chunk + (from_left ? 0 : 1)) * a.dim + at, acc);
         else put_grad<O, V>(out, a, id, at, acc);
     };
-    for (uint32_t c = c0; c < c1; c += U) {
-        uint32_t key[U];
-        float f[U][V];
+    for (uint32_t c = (uint32_t) c0; c < c1; c += U) {
+        uint32_t key[U], value[U];
+        WordOf<T, V> w[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const uint32_t i = min(c + u, c1 - 1);
             key[u] = a.keys[i];
-            if (key[u] < a.n) load<T, V>(grad + (uint64_t) a.values[i] * a.in_stride + at, f[u]);
+            value[u] = a.values[i];
         }
+#pragma unroll
+        for (int u = 0; u < U; u++) w[u] = get_word_if<WordOf<T, V>>(grad + (uint64_t) value[u] * a.in_stride + at, key[u] < a.n);
 #pragma unroll
         for (int u = 0; u < U; u++) {
             if (c + u >= c1) break;
@@ -324,67 +550,129 @@ __global__ void __launch_bounds__(256) grad_join_kernel(const T *__restrict__ gr
                 for (int i = 0; i < V; i++) acc[i] = 0.0f;
             }
             if (id < a.n) {
+                float f[V];
+                unpack<T, V>(w[u], f);
 #pragma unroll
-                for (int i = 0; i < V; i++) acc[i] += f[u][i];
+                for (int i = 0; i < V; i++) acc[i] += f[i];
             }
         }
     }
     put(c1 < a.items && a.keys[c1] == id);
 }
 
-// Runs over several chunks: whoever holds the chunk that a run starts in adds the partial sums in order.
+// Runs over several chunks: the CTA of the chunk that a run starts in adds its partial sums. Each of its eight warps takes an eighth of
+// the run's chunks, in order, and the warps' sums are added in order: the shape of the sum depends on the run alone.
 template<typename O, int V>
 __global__ void __launch_bounds__(256) grad_fix_kernel(O *__restrict__ out, GradArgs a) {
-    const uint32_t group = (blockIdx.x * 256 + threadIdx.x) / a.lanes, lane = threadIdx.x & (a.lanes - 1);
-    const uint32_t chunk = group / a.slabs, word = (group - chunk * a.slabs) * a.lanes + lane;
-    const uint32_t c0 = chunk * kChunk, c1 = c0 + kChunk;
-    if (c1 >= a.items || word >= a.words) return;
-    const uint32_t id = a.keys[c1 - 1], at = word * V;
+    __shared__ float part[8][32][V];
+    wait_for_previous();
+    const uint32_t chunk = blockIdx.x / a.slabs, slab = blockIdx.x - chunk * a.slabs;
+    const uint64_t c0 = (uint64_t) chunk * a.chunk, c1 = c0 + a.chunk;
+    if (c1 >= a.items) return;
+    const uint32_t id = a.keys[c1 - 1];
     if (id >= a.n || a.keys[c1] != id || (a.keys[c0] == id && c0 > 0 && a.keys[c0 - 1] == id)) return;
+    // the run's last chunk; the whole CTA is here
+    const uint32_t end = first_not_below(a.keys, (uint32_t) c1, a.items, id + 1), last = (end - 1) / a.chunk;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    const uint32_t word = slab * a.lanes + (lane & (a.lanes - 1)), at = word * V;
+    const bool mine = lane < a.lanes && word < a.words;
+    const uint32_t sums = last - chunk + 1, each = (sums + 7) / 8, s0 = min(warp * each, sums), s1 = min(s0 + each, sums);
     float acc[V];
-    load<float, V>(a.partial + (uint64_t) (2 * chunk + 1) * a.dim + at, acc);
-    for (uint32_t c = chunk + 1;; c++) {
-        float f[V];
-        load<float, V>(a.partial + (uint64_t) (2 * c) * a.dim + at, f);
 #pragma unroll
-        for (int i = 0; i < V; i++) acc[i] += f[i];
-        if ((c + 1) * kChunk >= a.items || a.keys[(c + 1) * kChunk] != id) break;
+    for (int i = 0; i < V; i++) acc[i] = 0.0f;
+    if (mine) {
+#pragma unroll 4
+        for (uint32_t s = s0; s < s1; s++) {
+            float f[V];
+            load<float, V>(a.partial + (2ull * (chunk + s) + (s == 0 ? 1 : 0)) * a.dim + at, f);
+#pragma unroll
+            for (int i = 0; i < V; i++) acc[i] += f[i];
+        }
+#pragma unroll
+        for (int i = 0; i < V; i++) part[warp][lane][i] = acc[i];
     }
+    __syncthreads();
+    if (warp != 0 || !mine) return;
+#pragma unroll
+    for (int w = 1; w < 8; w++)
+#pragma unroll
+        for (int i = 0; i < V; i++) acc[i] += part[w][lane][i];
     put_grad<O, V>(out, a, id, at, acc);
 }
 
 // ---- dispatch ---------------------------------------------------------------------------------------------------
-// A CTA places the pairs of a few rows (place = start of the partition + pairs of earlier tiles + rank in the tile), then copies
-// each of its rows, read once, to the places of its pairs.
-template<int B>
-__global__ void __launch_bounds__(256) dispatch_kernel(const uint8_t *__restrict__ rows, uint64_t stride, uint32_t count, uint32_t words,
-                                                       const uint32_t *__restrict__ choice, uint32_t choices, uint32_t partitions,
-                                                       const uint32_t *__restrict__ before, const uint32_t *__restrict__ totals,
-                                                       const uint16_t *__restrict__ ranks, uint32_t rows_each, uint8_t *__restrict__ sorted,
-                                                       uint64_t sorted_stride, uint32_t *__restrict__ position, uint32_t *__restrict__ map,
-                                                       uint32_t *__restrict__ segment_start) {
+// Each row, read once, is copied to the places of its pairs. A thread has U words of rows in flight.
+template<int B, int U>
+__global__ void __launch_bounds__(256) dispatch_kernel(const uint8_t *__restrict__ rows, uint64_t stride, uint32_t units, Div words, uint32_t choices,
+                                                       const uint32_t *__restrict__ position, uint8_t *__restrict__ sorted, uint64_t sorted_stride) {
     using W = typename Word<B>::type;
-    extern __shared__ uint32_t smem[];
-    uint32_t *starts = smem, *place = smem + partitions + 1;
-    bucket_starts<256>(totals, partitions + 1, starts);
-    if (blockIdx.x == 0)
-        for (uint32_t i = threadIdx.x; i <= partitions; i += 256) segment_start[i] = starts[i];
-    const uint32_t r0 = blockIdx.x * rows_each, nr = min(rows_each, count - r0);
-    for (uint32_t i = threadIdx.x; i < nr * choices; i += 256) {
-        const uint32_t pair = r0 * choices + i, e = min(choice[pair], partitions);
-        const uint32_t p = starts[e] + before[(uint64_t) (pair / kTile) * (partitions + 1) + e] + ranks[pair];
-        const bool there = e < partitions;
-        place[i] = there ? p : kNone;
-        position[pair] = there ? p : kNone;
-        map[p] = there ? pair / choices : kNone;   // pairs without a partition come last: their places are the tail
+    const uint32_t first = blockIdx.x * (256 * U) + threadIdx.x;
+    uint32_t row[U], at[U];
+    W w[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const uint32_t x = min(first + u * 256, units - 1);
+        row[u] = words.of(x);
+        at[u] = (x - row[u] * words.d) * B;
+        w[u] = get_word<false>(reinterpret_cast<const W *>(rows + (uint64_t) row[u] * stride + at[u]));
+    }
+    wait_for_previous();   // the places come from the launch before, the rows do not
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        if (first + u * 256 >= units) break;
+#pragma unroll 4
+        for (uint32_t j = 0; j < choices; j++) {
+            const uint32_t p = position[(uint64_t) row[u] * choices + j];
+            if (p != kNone) put_word(reinterpret_cast<W *>(sorted + (uint64_t) p * sorted_stride + at[u]), w[u]);
+        }
+    }
+}
+
+// Few pairs: everything in one launch. A CTA owns one row; a warp finds a pair's place by comparing it with all pairs (at most
+// kSmallPairs of them, in shared memory), then the CTA copies the row. One CTA more counts the partitions.
+template<int B>
+__global__ void __launch_bounds__(256) dispatch_small_kernel(const uint8_t *__restrict__ rows, uint64_t stride, uint32_t count, uint32_t words,
+                                                             const uint32_t *__restrict__ choice, uint32_t choices, uint32_t partitions,
+                                                             uint8_t *__restrict__ sorted, uint64_t sorted_stride, uint32_t *__restrict__ position,
+                                                             uint32_t *__restrict__ map, uint32_t *__restrict__ segment_start) {
+    using W = typename Word<B>::type;
+    __shared__ uint32_t keys[kSmallPairs], place[kMaxChoices];
+    extern __shared__ __align__(16) uint32_t counts[];
+    const uint32_t pairs = count * choices, warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, row = blockIdx.x;
+    if (row == count) {
+        for (uint32_t b = threadIdx.x; b <= partitions; b += 256) counts[b] = 0;
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < pairs; i += 256) {
+            const uint32_t e = choice[i];
+            if (e < partitions) atomicAdd(counts + e, 1u);
+        }
+        scan_buckets(counts, partitions + 1);
+        for (uint32_t b = threadIdx.x; b <= partitions; b += 256) segment_start[b] = counts[b];
+        return;
+    }
+    for (uint32_t i = threadIdx.x; i < pairs; i += 256) keys[i] = min(choice[i], partitions);
+    W w;
+    memset(&w, 0, sizeof w);
+    const uint8_t *from = rows + (uint64_t) row * stride;
+    if (threadIdx.x < words) w = get_word<false>(reinterpret_cast<const W *>(from + (uint64_t) threadIdx.x * B));
+    __syncthreads();
+    for (uint32_t j = warp; j < choices; j += 8) {
+        const uint32_t pair = row * choices + j, key = keys[pair];
+        uint32_t before = 0;
+        for (uint32_t i = lane; i < pairs; i += 32) before += keys[i] < key || (keys[i] == key && i < pair);
+        before = __reduce_add_sync(0xffffffffu, before);
+        if (lane == 0) {
+            const bool there = key < partitions;
+            place[j] = position[pair] = there ? before : kNone;
+            map[before] = there ? row : kNone;
+        }
     }
     __syncthreads();
-    for (uint32_t x = threadIdx.x; x < nr * words; x += 256) {
-        const uint32_t r = x / words, c = x - r * words;
-        const W w = *reinterpret_cast<const W *>(rows + (uint64_t) (r0 + r) * stride + (uint64_t) c * B);
+    for (uint32_t c = threadIdx.x; c < words; c += 256) {
+        if (c != threadIdx.x) w = get_word<false>(reinterpret_cast<const W *>(from + (uint64_t) c * B));
         for (uint32_t j = 0; j < choices; j++) {
-            const uint32_t p = place[r * choices + j];
-            if (p != kNone) *reinterpret_cast<W *>(sorted + (uint64_t) p * sorted_stride + (uint64_t) c * B) = w;
+            const uint32_t p = place[j];
+            if (p != kNone) put_word(reinterpret_cast<W *>(sorted + (uint64_t) p * sorted_stride + (uint64_t) c * B), w);
         }
     }
 }
@@ -404,7 +692,8 @@ __global__ void __launch_bounds__(256) combine_kernel(const T *__restrict__ sort
     for (int i = 0; i < V; i++) acc[i] = 0.0f;
     for (uint32_t j0 = 0; j0 < choices; j0 += K) {
         uint32_t p[K];
-        float w[K], f[K][V];
+        float w[K];
+        WordOf<T, V> y[K];
 #pragma unroll
         for (int j = 0; j < K; j++) {
             const uint64_t pair = (uint64_t) row * choices + j0 + j;
@@ -412,13 +701,14 @@ __global__ void __launch_bounds__(256) combine_kernel(const T *__restrict__ sort
             w[j] = weights && j0 + j < choices ? weights[pair] : 1.0f;
         }
 #pragma unroll
-        for (int j = 0; j < K; j++)
-            if (p[j] < sorted_rows) load<T, V>(sorted + (uint64_t) p[j] * stride + at, f[j]);
+        for (int j = 0; j < K; j++) y[j] = get_word_if<WordOf<T, V>>(sorted + (uint64_t) p[j] * stride + at, p[j] < sorted_rows);
 #pragma unroll
         for (int j = 0; j < K; j++) {
             if (p[j] >= sorted_rows) continue;
+            float f[V];
+            unpack<T, V>(y[j], f);
 #pragma unroll
-            for (int i = 0; i < V; i++) acc[i] = fmaf(w[j], f[j][i], acc[i]);
+            for (int i = 0; i < V; i++) acc[i] = fmaf(w[j], f[i], acc[i]);
         }
     }
     store<T, V>(out + (uint64_t) row * out_stride + at, acc);
@@ -445,18 +735,19 @@ __global__ void __launch_bounds__(256) combine_grad_kernel(const T *__restrict__
             dot[j] = 0.0f;
         }
         for (uint32_t c = l; c < words; c += G) {
-            float g[V], f[K][V];
-            load<T, V>(grad + (uint64_t) row * grad_stride + (uint64_t) c * V, g);
+            float g[V];
+            WordOf<T, V> y[K];
 #pragma unroll
-            for (int j = 0; j < K; j++)
-                if (p[j] < sorted_rows) load<T, V>(sorted + (uint64_t) p[j] * stride + (uint64_t) c * V, f[j]);
+            for (int j = 0; j < K; j++) y[j] = get_word_if<WordOf<T, V>>(sorted + (uint64_t) p[j] * stride + (uint64_t) c * V, p[j] < sorted_rows);
+            load<T, V>(grad + (uint64_t) row * grad_stride + (uint64_t) c * V, g);
 #pragma unroll
             for (int j = 0; j < K; j++) {
                 if (p[j] >= sorted_rows) continue;
-                float o[V];
+                float f[V], o[V];
+                unpack<T, V>(y[j], f);
 #pragma unroll
                 for (int i = 0; i < V; i++) {
-                    dot[j] = fmaf(g[i], f[j][i], dot[j]);
+                    dot[j] = fmaf(g[i], f[i], dot[j]);
                     o[i] = w[j] * g[i];
                 }
                 store<T, V>(grad_sorted + (uint64_t) p[j] * grad_sorted_stride + (uint64_t) c * V, o);
@@ -591,17 +882,24 @@ cudaError_t launch_lookup(const void *table, uint64_t table_stride, uint32_t n, 
     return cudaSuccess;
 }
 
-// Shared memory of the counting kernel: above the 48 KB that need no word from the launcher for many buckets.
-cudaError_t launch_count(const uint32_t *keys, uint32_t items, Digit digit, uint32_t buckets, uint32_t *counts, uint16_t *ranks,
-                         uint32_t *totals, cudaStream_t stream) {
-    const uint32_t tiles = (uint32_t) ceil_div(items, kTile), smem = kSortWarps * buckets * 2;
-    if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(bucket_count_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem);
-        if (e != cudaSuccess) return e;
-    }
-    bucket_count_kernel<<<tiles, kSortThreads, smem, stream>>>(keys, items, digit, buckets, counts, ranks);
-    bucket_scan_kernel<<<(uint32_t) ceil_div(buckets, 32), 1024, 0, stream>>>(counts, tiles, buckets, totals);
-    return cudaGetLastError();
+// The shape of a counting sort: 1,024 threads a CTA, 512 where the counters of 32 warps would not fit.
+struct Tiles {
+    uint32_t threads, items, count;
+    Tiles(uint64_t all, uint32_t buckets) : threads(buckets > (1u << kMaxPassBits) ? 512 : 1024), items(threads * kRounds), count((uint32_t) ceil_div(all, items)) {}
+};
+
+// One pass over more than one tile.
+template<typename To>
+cudaError_t sort_pass(const uint32_t *keys, uint32_t items, const Digit &digit, uint32_t buckets, uint32_t *counts, uint32_t *totals, uint16_t *ranks,
+                      const To &to, bool dependent, cudaStream_t stream) {
+    const Tiles t(items, buckets);
+    cudaError_t e = launch(bucket_count_kernel, t.count, t.threads, rank_smem(t.threads / 32, buckets), stream, dependent, keys, items, digit, buckets, counts, ranks);
+    if (e != cudaSuccess) return e;
+    if (t.count <= kMaxFusedTiles)
+        return launch(bucket_place_kernel<To, false>, t.count, t.threads, buckets * 4, stream, true, keys, items, digit, buckets, counts, t.count, totals, ranks, to);
+    e = launch(bucket_scan_kernel, ceil_div(buckets, 32), 1024, 0, stream, true, counts, t.count, buckets, totals);
+    if (e != cudaSuccess) return e;
+    return launch(bucket_place_kernel<To, true>, t.count, t.threads, buckets * 4, stream, true, keys, items, digit, buckets, counts, t.count, totals, ranks, to);
 }
 
 // Scratch of the gradient: two copies of the sorted items, the counts of a pass, the partial sums of its chunks.
@@ -609,47 +907,47 @@ struct GradScratch {
     uint32_t *keys[2], *values[2], *counts, *totals;
     uint16_t *ranks;
     float *partial;
-    uint32_t bits, passes, pass_bits;
+    uint32_t bits, passes, pass_bits, chunk;
     uint64_t bytes;
     GradScratch(void *base, uint64_t n, uint64_t items, uint32_t dim) {
         bits = 1;
         while ((1ull << bits) <= n) bits++;             // ids 0 .. n - 1, and n for none
-        passes = (bits + 10) / 11;
+        passes = (bits + kMaxPassBits - 1) / kMaxPassBits;
         pass_bits = (bits + passes - 1) / passes;
+        chunk = 32;
         uint64_t at = 0;
         auto take = [&](uint64_t size) {
             const uint64_t here = at;
             at += align256(size);
             return static_cast<char *>(base) + here;
         };
-        const uint64_t tiles = ceil_div(items, kTile);
         for (int i = 0; i < 2; i++) {
             keys[i] = reinterpret_cast<uint32_t *>(take(items * 4));
             values[i] = reinterpret_cast<uint32_t *>(take(items * 4));
         }
         ranks = reinterpret_cast<uint16_t *>(take(items * 2));
-        counts = reinterpret_cast<uint32_t *>(take((tiles << pass_bits) * 4));
+        counts = reinterpret_cast<uint32_t *>(take(((uint64_t) Tiles(items, 1u << pass_bits).count << pass_bits) * 4));
         totals = reinterpret_cast<uint32_t *>(take(4ull << pass_bits));
-        partial = reinterpret_cast<float *>(take(2 * ceil_div(items, kChunk) * dim * 4));
+        partial = reinterpret_cast<float *>(take(2 * ceil_div(items, chunk) * dim * 4));
         bytes = at;
     }
 };
 
 struct DispatchScratch {
-    uint32_t *counts, *totals;
-    uint16_t *ranks;
-    uint64_t bytes;
+    uint32_t *counts = nullptr, *totals = nullptr;
+    uint16_t *ranks = nullptr;
+    uint64_t bytes = 0;
     DispatchScratch(void *base, uint64_t pairs, uint32_t partitions) {
-        uint64_t at = 0;
+        const Tiles t(pairs, partitions + 1);
+        if (pairs <= kSmallPairs || t.count <= 1) return;
         auto take = [&](uint64_t size) {
-            const uint64_t here = at;
-            at += align256(size);
+            const uint64_t here = bytes;
+            bytes += align256(size);
             return static_cast<char *>(base) + here;
         };
         ranks = reinterpret_cast<uint16_t *>(take(pairs * 2));
-        counts = reinterpret_cast<uint32_t *>(take(ceil_div(pairs, kTile) * (partitions + 1) * 4));
+        counts = reinterpret_cast<uint32_t *>(take((uint64_t) t.count * (partitions + 1) * 4));
         totals = reinterpret_cast<uint32_t *>(take((partitions + 1) * 4ull));
-        bytes = at;
     }
 };
 
@@ -709,34 +1007,41 @@ int glide_lookup_rows_grad(glide_ctx *ctx, const void *d_grad, int row_type, uin
     const OnDevice guard(ctx->device);
     ROWS_CUDA(guard.status);
     auto s = static_cast<cudaStream_t>(stream);
-    if (!accumulate)
-        ROWS_CUDA(cudaMemset2DAsync(d_table_grad, table_grad_stride * bytes_of(grad_type), 0, (size_t) dim * bytes_of(grad_type), n, s));
-    if (count == 0) return GLIDE_OK;
     const GradScratch w(d_workspace, n, count, dim);
     const uint32_t items = (uint32_t) count;
     const uint32_t *keys = d_ids, *values = nullptr;
-    for (uint32_t pass = 0; pass < w.passes; pass++) {
-        const uint32_t left = w.bits - pass * w.pass_bits, here = left < w.pass_bits ? left : w.pass_bits, buckets = 1u << here;
-        const Digit digit{(uint32_t) n, pass * w.pass_bits, buckets - 1};
-        ROWS_CUDA(launch_count(keys, items, digit, buckets, w.counts, w.ranks, w.totals, s));
-        bucket_scatter_kernel<<<(uint32_t) ceil_div(items, kTile), kSortThreads, buckets * 4, s>>>(keys, values, items, digit, buckets, w.counts, w.totals, w.ranks, w.keys[pass & 1], w.values[pass & 1]);
-        ROWS_CUDA(cudaGetLastError());
-        keys = w.keys[pass & 1];
-        values = w.values[pass & 1];
+    if (count > 0 && Tiles(items, 1u << w.pass_bits).count == 1) {
+        const uint32_t threads = (uint32_t) ceil_div(items, kRounds * 32) * 32, last = (w.passes - 1) & 1;
+        ROWS_CUDA(launch(sort_tile_kernel, 1, threads, rank_smem(threads / 32, 1u << w.pass_bits) + (4u << w.pass_bits), s, false, d_ids, items, (uint32_t) n, w.bits, w.pass_bits,
+                         w.keys[0], w.values[0], w.keys[1], w.values[1]));
+        keys = w.keys[last];
+        values = w.values[last];
+    } else if (count > 0) {
+        for (uint32_t pass = 0; pass < w.passes; pass++) {
+            const uint32_t left = w.bits - pass * w.pass_bits, here = left < w.pass_bits ? left : w.pass_bits, buckets = 1u << here;
+            ROWS_CUDA(sort_pass(keys, items, Digit{(uint32_t) n, pass * w.pass_bits, buckets - 1}, buckets, w.counts, w.totals, w.ranks, ToSorted{values, w.keys[pass & 1], w.values[pass & 1]}, pass > 0, s));
+            keys = w.keys[pass & 1];
+            values = w.values[pass & 1];
+        }
     }
-    const uint32_t most = most_of(row_type), v0 = in.width(most), v1 = out.width(most), v = v0 < v1 ? v0 : v1;
-    GradArgs a{keys, values, items, (uint32_t) n, dim, dim / v, 32, 1, scale, grad_stride, table_grad_stride, accumulate, w.partial};
+    const uint32_t most = most_of(row_type), v0 = count ? in.width(most) : most, v1 = out.width(most), v = v0 < v1 ? v0 : v1;
+    GradArgs a{keys, values, items, (uint32_t) n, dim, dim / v, 32, 1, w.chunk, scale, grad_stride, table_grad_stride, accumulate, w.partial, 0, 0};
     while (a.lanes > 1 && a.lanes / 2 >= a.words) a.lanes /= 2;
     a.slabs = (uint32_t) ceil_div(a.words, a.lanes);
-    const uint64_t grid = ceil_div(ceil_div(items, kChunk) * a.slabs * a.lanes, 256);
-    ROWS_REQUIRE(grid <= 0xffffffu, GLIDE_ERR_UNSUPPORTED, "lookup_rows_grad: too many values in one call");   // threads are counted in 32 bits
+    const uint64_t chunks = ceil_div(items, a.chunk), join = ceil_div(chunks * a.slabs * a.lanes, 256);
+    a.zero_rows = (128u << 10) / (dim * bytes_of(grad_type));   // a CTA clears up to 128 KB
+    a.zero_rows = a.zero_rows < 1 ? 1 : a.zero_rows > 256 ? 256 : a.zero_rows;
+    const uint64_t zero = accumulate ? 0 : ceil_div(n, a.zero_rows);
+    ROWS_REQUIRE(join <= 0xffffffu && chunks * a.slabs <= 0x7fffffffu && join + zero <= 0x7fffffffu, GLIDE_ERR_UNSUPPORTED, "lookup_rows_grad: too many values in one call");   // threads are counted in 32 bits
+    a.join_blocks = (uint32_t) join;
+    if (join + zero == 0) return GLIDE_OK;
     auto run = [&](auto t, auto o, auto wd) {
         using T = decltype(t);
         using O = decltype(o);
         constexpr int V = decltype(wd)::value;
-        grad_join_kernel<T, O, V><<<(uint32_t) grid, 256, 0, s>>>(static_cast<const T *>(d_grad), static_cast<O *>(d_table_grad), a);
-        grad_fix_kernel<O, V><<<(uint32_t) grid, 256, 0, s>>>(static_cast<O *>(d_table_grad), a);
-        return cudaGetLastError();
+        const cudaError_t e = launch(grad_join_kernel<T, O, V>, join + zero, 256, 0, s, count > 0, static_cast<const T *>(d_grad), static_cast<O *>(d_table_grad), a);
+        if (e != cudaSuccess || chunks < 2) return e;
+        return launch(grad_fix_kernel<O, V>, (chunks - 1) * a.slabs, 256, 0, s, true, static_cast<O *>(d_table_grad), a);
     };
     ROWS_CUDA(with_rows(row_type, v, [&](auto t, auto wd) { return grad_type == GLIDE_ROW_F32 ? run(t, float{}, wd) : run(t, t, wd); }));
     return GLIDE_OK;
@@ -776,24 +1081,44 @@ int glide_dispatch_rows(glide_ctx *ctx, const void *d_rows, int row_type, uint64
         ROWS_CUDA(cudaMemsetAsync(d_segment_start, 0, (partitions + 1) * 4ull, s));
         return GLIDE_OK;
     }
-    const DispatchScratch w(d_workspace, pairs, partitions);
-    ROWS_CUDA(launch_count(d_choice, (uint32_t) pairs, Digit{partitions, 0, kNone}, partitions + 1, w.counts, w.ranks, w.totals, s));
     const uint32_t e = bytes_of(row_type), most = 16 / e, v0 = in.width(most), v1 = out.width(most), v = v0 < v1 ? v0 : v1, words = dim / v;
-    uint32_t each = 2048 / words;   // rows of a CTA: some 2,048 words to copy, and as many pairs at most
-    if (each > 2048 / choices) each = 2048 / choices;
-    if (each < 1) each = 1;
-    if (each > count) each = (uint32_t) count;
-    const uint32_t grid = (uint32_t) ceil_div(count, each), smem = (partitions + 1 + each * choices) * 4;
-    auto run = [&](auto b) {
-        dispatch_kernel<decltype(b)::value><<<grid, 256, smem, s>>>(static_cast<const uint8_t *>(d_rows), row_stride * e, (uint32_t) count, words, d_choice, choices, partitions, w.counts, w.totals, w.ranks, each,
-                                                                   static_cast<uint8_t *>(d_sorted), sorted_stride * e, d_position, d_map, d_segment_start);
-        return cudaGetLastError();
+    const uint8_t *from = static_cast<const uint8_t *>(d_rows);
+    uint8_t *to = static_cast<uint8_t *>(d_sorted);
+    auto with_bytes = [&](auto run) {
+        switch (v * e) {
+            case 16: return run(Width<16>{});
+            case 8: return run(Width<8>{});
+            case 4: return run(Width<4>{});
+            default: return run(Width<2>{});
+        }
     };
-    switch (v * e) {
-        case 16: ROWS_CUDA(run(Width<16>{})); break;
-        case 8: ROWS_CUDA(run(Width<8>{})); break;
-        case 4: ROWS_CUDA(run(Width<4>{})); break;
-        default: ROWS_CUDA(run(Width<2>{})); break;
+    if (pairs <= kSmallPairs) {
+        ROWS_CUDA(with_bytes([&](auto b) {
+            return launch(dispatch_small_kernel<decltype(b)::value>, count + 1, 256, (partitions + 1) * 4, s, false, from, row_stride * e, (uint32_t) count, words, d_choice, choices, partitions,
+                          to, sorted_stride * e, d_position, d_map, d_segment_start);
+        }));
+        return GLIDE_OK;
+    }
+    const DispatchScratch w(d_workspace, pairs, partitions);
+    const Tiles tiles(pairs, partitions + 1);
+    const Digit digit{partitions, 0, kNone};
+    const ToPlaces places{d_position, d_map, d_segment_start, Div(choices)};
+    if (tiles.count == 1) {
+        const uint32_t threads = (uint32_t) ceil_div(pairs, kRounds * 32) * 32;
+        ROWS_CUDA(launch(place_tile_kernel, 1, threads, rank_smem(threads / 32, partitions + 1) + (partitions + 1) * 4, s, false, d_choice, (uint32_t) pairs, digit, partitions + 1, places));
+    } else {
+        ROWS_CUDA(sort_pass(d_choice, (uint32_t) pairs, digit, partitions + 1, w.counts, w.totals, w.ranks, places, false, s));
+    }
+    const uint64_t each = 0x7fff0000u / words;   // rows of a launch: its words are counted in 31 bits
+    for (uint64_t r0 = 0; r0 < count; r0 += each) {
+        const uint32_t rows = (uint32_t) (count - r0 < each ? count - r0 : each), units = rows * words;
+        ROWS_CUDA(with_bytes([&](auto b) {
+            constexpr int B = decltype(b)::value;
+            const uint8_t *part = from + r0 * row_stride * e;
+            const uint32_t *position = d_position + r0 * choices;
+            if (units <= 256 * 1024) return launch(dispatch_kernel<B, 1>, ceil_div(units, 256), 256, 0, s, r0 == 0, part, row_stride * e, units, Div(words), choices, position, to, sorted_stride * e);
+            return launch(dispatch_kernel<B, 4>, ceil_div(units, 1024), 256, 0, s, r0 == 0, part, row_stride * e, units, Div(words), choices, position, to, sorted_stride * e);
+        }));
     }
     return GLIDE_OK;
 }

@@ -605,7 +605,7 @@ def test_c_entry_points_refuse_what_they_do_not_take(gpu_ctx):
     send(BAD, p=I)
     send(BAD, mp=J)
     send(BAD, out=X)
-    send(BAD, wb=10)
+    send(BAD, count=10_000, wb=10)        # few pairs need no workspace, these do
     send(BAD, os=8)
     send(BAD, w=W + 8)
 

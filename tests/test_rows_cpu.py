@@ -89,7 +89,7 @@ def test_workspaces_hold_what_the_calls_need():
         for count in (1, 31, 2049, 1 << 20):
             assert lib.glide_lookup_rows_grad_workspace(n, 128, count) >= 18 * count
     assert lib.glide_lookup_rows_grad_workspace(100, 128, 0) == 0
-    assert lib.glide_dispatch_rows_workspace(1000, 8, 64) >= 2 * 8000
+    assert lib.glide_dispatch_rows_workspace(100_000, 8, 64) >= 2 * 800_000
     # what the calls refuse needs no workspace
     assert lib.glide_dispatch_rows_workspace(1000, 129, 64) == 0
     assert lib.glide_dispatch_rows_workspace(1000, 8, 4097) == 0
