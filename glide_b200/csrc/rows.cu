@@ -25,8 +25,11 @@ constexpr uint32_t kMaxPartitions = 4096;   // of dispatch_rows: a counter for e
 constexpr uint32_t kMaxChoices = 128;       // as many as glide_bruteforce_knn returns neighbours
 constexpr uint32_t kMaxDim = 1u << 20;
 constexpr uint32_t kRounds = 8;             // items of a thread in the counting sort
-constexpr uint32_t kMaxPassBits = 11;       // digits of a pass: 32 warps' counters take 128 KB of shared memory
+constexpr uint32_t kTileThreads = 256, kTile = kTileThreads * kRounds;
+constexpr uint32_t kOneTile = 4096;         // items that one CTA sorts in one launch
+constexpr uint32_t kMaxPassBits = 11;       // digits of a pass: the counters of kOneTile's 16 warps take 64 KB of shared memory
 constexpr uint32_t kMaxFusedTiles = 64;     // tiles whose counts every CTA of the second kernel adds up by itself
+constexpr uint32_t kClearShare = 24u << 20; // bytes of a gradient that are cleared beside each launch of its sort
 constexpr uint32_t kSmallPairs = 2048;      // pairs that dispatch_rows places and copies in one launch
 
 // ---- rows as words ----------------------------------------------------------------------------------------
@@ -157,9 +160,10 @@ __global__ void __launch_bounds__(256) lookup_kernel(const T *__restrict__ table
 // ---- launches that follow one another -----------------------------------------------------------------------------
 // The kernels of one call are launched as programmatic dependents: the next one's CTAs become resident while the last one
 // drains, and wait() holds them until everything before is complete and visible.
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_previous() {
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    let_next_start();
 }
 
 template<typename... P, typename... A>
@@ -185,35 +189,80 @@ cudaError_t launch(void (*kernel)(P...), uint64_t grid, uint32_t block, uint32_t
 // One pass places every item behind all items of a smaller digit and behind the items of its own digit that came before it.
 // A CTA takes a tile of consecutive items, each of its warps a run of 256, 32 at a time: a lane's rank among the items of
 // its digit is the warp's running count plus the equal digits at lower lanes, and a scan over the warps' counts makes it the
-// rank in the tile. No atomics: the order depends on nothing but the keys. Few launches count most here (the data are 6 bytes
-// an item): one tile is sorted by one launch, up to kMaxFusedTiles by two launches a pass (every CTA of the second adds up
-// the counts of all tiles), more by three.
+// rank in the tile. No atomics: the order depends on nothing but the keys. Few launches count most here (the data are 6 to 10
+// bytes an item): kOneTile items are sorted by one launch, up to kMaxFusedTiles tiles by two launches a pass (every CTA of the
+// second adds up the counts of all tiles), more by three. Tiles are small because their items' scattered stores leave an SM at
+// one sector a cycle: with 8,192 items to a tile a pass over 100,000 ids took 31 us.
 struct Digit {
-    uint32_t limit, shift, mask;   // keys beyond limit count as limit
-    __device__ __forceinline__ uint32_t of(uint32_t key) const { return (min(key, limit) >> shift) & mask; }
+    uint32_t limit, shift, bits;   // keys beyond limit count as limit; bits: of the digit
+    __device__ __forceinline__ uint32_t of(uint32_t key) const { return (min(key, limit) >> shift) & ((1u << bits) - 1); }
 };
 
-__device__ __forceinline__ uint32_t warp_items() { return kRounds * 32; }
+// Keys alone, or in the first half of items that an earlier pass has placed (the second: an item's value).
+struct Keys {
+    const uint32_t *plain;
+    const uint2 *items;
+    __device__ __forceinline__ uint2 item(uint32_t i) const { return items ? items[i] : make_uint2(plain[i], i); }
+    __device__ __forceinline__ uint32_t key(uint32_t i) const { return items ? items[i].x : plain[i]; }
+};
+
+// Rows that CTAs without a tile clear while the others sort (bytes of memory that is idle then).
+struct Clear {
+    uint8_t *at;
+    uint64_t stride, bytes;    // of a row
+    uint32_t rows, each;       // all rows, and those of a CTA
+    uint32_t word;             // 16, 4 or 2: what addresses, strides and bytes are multiples of
+    __host__ __device__ uint32_t blocks() const { return rows == 0 ? 0 : (rows - 1) / each + 1; }
+    template<typename W> __device__ __forceinline__ void run(uint32_t r0, uint32_t r1) const {
+        const uint32_t words = (uint32_t) (bytes / sizeof(W));
+        W zero;
+        memset(&zero, 0, sizeof zero);
+        for (uint32_t x = threadIdx.x; x < (r1 - r0) * words; x += blockDim.x) {
+            const uint32_t r = x / words, w = x - r * words;
+            __stcg(reinterpret_cast<W *>(at + (r0 + r) * stride) + w, zero);
+        }
+    }
+    // Touches nothing that the launches before it read or write, so it waits for none of them.
+    __device__ __forceinline__ void block(uint32_t b) const {
+        let_next_start();
+        const uint32_t r0 = b * each, r1 = min(r0 + each, rows);
+        if (word == 16) run<uint4>(r0, r1);
+        else if (word == 4) run<uint32_t>(r0, r1);
+        else run<uint16_t>(r0, r1);
+    }
+};
+
 __device__ __forceinline__ uint32_t tile_item(uint32_t r) {   // of this thread, from the tile's first
-    return (threadIdx.x >> 5) * warp_items() + r * 32 + (threadIdx.x & 31u);
+    return (threadIdx.x >> 5) * (kRounds * 32) + r * 32 + (threadIdx.x & 31u);
 }
 
 // Ranks in the tile of this thread's items by their digits (kNone: no item), and the tile's count of each bucket through `put`.
+// Lanes of the same digit are found by a ballot for each bit (a match instruction took twice as long).
 template<typename Put>
-__device__ __forceinline__ void rank_tile(const uint32_t (&d)[kRounds], uint32_t buckets, uint16_t *warp_counts, uint32_t (&rank)[kRounds], Put put) {
+__device__ __forceinline__ void rank_tile(const uint32_t (&d)[kRounds], uint32_t bits, uint32_t buckets, uint16_t *warp_counts, uint32_t (&rank)[kRounds], Put put) {
     const uint32_t warps = blockDim.x >> 5, lane = threadIdx.x & 31u;
     const uint32_t words = (warps * buckets + 7) / 8;
     for (uint32_t i = threadIdx.x; i < words; i += blockDim.x) reinterpret_cast<uint4 *>(warp_counts)[i] = make_uint4(0, 0, 0, 0);
+    uint32_t same[kRounds];
+#pragma unroll
+    for (uint32_t r = 0; r < kRounds; r++) same[r] = __ballot_sync(0xffffffffu, d[r] != kNone);
+    for (uint32_t b = 0; b < bits; b++) {
+#pragma unroll
+        for (uint32_t r = 0; r < kRounds; r++) {
+            const bool set = d[r] >> b & 1u;
+            const uint32_t others = __ballot_sync(0xffffffffu, set);
+            same[r] &= set ? others : ~others;
+        }
+    }
     __syncthreads();
     uint16_t *mine = warp_counts + (threadIdx.x >> 5) * buckets;
 #pragma unroll
     for (uint32_t r = 0; r < kRounds; r++) {
-        const uint32_t same = __match_any_sync(0xffffffffu, d[r]);
         const bool there = d[r] != kNone;
         const uint32_t before = there ? mine[d[r]] : 0;
-        rank[r] = before + __popc(same & ((1u << lane) - 1));
+        rank[r] = before + __popc(same[r] & ((1u << lane) - 1));
         __syncwarp();
-        if (there && (same >> lane) == 1u) mine[d[r]] = (uint16_t) (before + __popc(same));
+        if (there && (same[r] >> lane) == 1u) mine[d[r]] = (uint16_t) (before + __popc(same[r]));
         __syncwarp();
     }
     __syncthreads();
@@ -240,10 +289,16 @@ __device__ __forceinline__ void scan_buckets(uint32_t *values, uint32_t buckets)
     __shared__ uint32_t all;
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     uint32_t carry = 0;
-    for (uint32_t b0 = 0; b0 < buckets; b0 += blockDim.x) {
+    for (uint32_t b0 = 0; b0 < buckets; b0 += blockDim.x * 4) {
         __syncthreads();
-        const uint32_t b = b0 + threadIdx.x, v = b < buckets ? values[b] : 0;
-        uint32_t incl = v;
+        const uint32_t b = b0 + threadIdx.x * 4;
+        uint32_t v[4], sum = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            v[i] = b + i < buckets ? values[b + i] : 0;
+            sum += v[i];
+        }
+        uint32_t incl = sum;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
             const uint32_t o = __shfl_up_sync(0xffffffffu, incl, off);
@@ -252,31 +307,31 @@ __device__ __forceinline__ void scan_buckets(uint32_t *values, uint32_t buckets)
         if (lane == 31) warp_sum[warp] = incl;
         __syncthreads();
         if (warp == 0) {
-            uint32_t w = lane < warps ? warp_sum[lane] : 0, sum = w;
+            uint32_t w = lane < warps ? warp_sum[lane] : 0, run = w;
 #pragma unroll
             for (int off = 1; off < 32; off <<= 1) {
-                const uint32_t o = __shfl_up_sync(0xffffffffu, sum, off);
-                if (lane >= (uint32_t) off) sum += o;
+                const uint32_t o = __shfl_up_sync(0xffffffffu, run, off);
+                if (lane >= (uint32_t) off) run += o;
             }
-            warp_sum[lane] = sum - w;
-            if (lane == 31) all = sum;
+            warp_sum[lane] = run - w;
+            if (lane == 31) all = run;
         }
         __syncthreads();
-        if (b < buckets) values[b] = carry + warp_sum[warp] + incl - v;
+        uint32_t run = carry + warp_sum[warp] + incl - sum;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (b + i < buckets) values[b + i] = run;
+            run += v[i];
+        }
         carry += all;
     }
     __syncthreads();
 }
 
-// Where a pass leaves its items. Radix: keys and values in their new order; values_in == nullptr: an item's value is its index.
+// Where a pass leaves its items. A radix sort: key and value in their new order.
 struct ToSorted {
-    const uint32_t *values_in;
-    uint32_t *keys, *values;
-    __device__ __forceinline__ uint32_t value_of(uint32_t i) const { return values_in ? values_in[i] : i; }
-    __device__ __forceinline__ void item(uint32_t, uint32_t value, uint32_t key, const Digit &, uint32_t place) const {
-        keys[place] = key;
-        values[place] = value;
-    }
+    uint2 *items;
+    __device__ __forceinline__ void item(uint2 item, const Digit &digit, uint32_t place) const { items[place] = make_uint2(min(item.x, digit.limit), item.y); }
     __device__ __forceinline__ void start(uint32_t, uint32_t) const {}
 };
 
@@ -285,28 +340,28 @@ struct ToSorted {
 struct ToPlaces {
     uint32_t *position, *map, *segment_start;
     Div choices;
-    __device__ __forceinline__ uint32_t value_of(uint32_t i) const { return i; }
-    __device__ __forceinline__ void item(uint32_t pair, uint32_t, uint32_t key, const Digit &digit, uint32_t place) const {
-        const bool there = key < digit.limit;
-        position[pair] = there ? place : kNone;
-        map[place] = there ? choices.of(pair) : kNone;
+    __device__ __forceinline__ void item(uint2 item, const Digit &digit, uint32_t place) const {
+        const bool there = item.x < digit.limit;
+        position[item.y] = there ? place : kNone;
+        map[place] = there ? choices.of(item.y) : kNone;
     }
     __device__ __forceinline__ void start(uint32_t bucket, uint32_t place) const { segment_start[bucket] = place; }
 };
 
-__global__ void __launch_bounds__(1024) bucket_count_kernel(const uint32_t *__restrict__ keys, uint32_t items, Digit digit, uint32_t buckets,
-                                                            uint32_t *__restrict__ counts, uint16_t *__restrict__ ranks) {
+__global__ void __launch_bounds__(kTileThreads) bucket_count_kernel(Keys keys, uint32_t items, Digit digit, uint32_t buckets, uint32_t tiles,
+                                                                    uint32_t *__restrict__ counts, uint16_t *__restrict__ ranks, Clear clear) {
     extern __shared__ __align__(16) uint16_t warp_counts[];
+    if (blockIdx.x >= tiles) return clear.block(blockIdx.x - tiles);
     wait_for_previous();
-    const uint32_t first = blockIdx.x * (blockDim.x * kRounds);
+    const uint32_t first = blockIdx.x * kTile;
     uint32_t d[kRounds], rank[kRounds];
 #pragma unroll
     for (uint32_t r = 0; r < kRounds; r++) {
         const uint32_t i = first + tile_item(r);
-        d[r] = i < items ? digit.of(keys[i]) : kNone;
+        d[r] = i < items ? digit.of(keys.key(i)) : kNone;
     }
     uint32_t *mine = counts + (uint64_t) blockIdx.x * buckets;
-    rank_tile(d, buckets, warp_counts, rank, [&](uint32_t b, uint32_t sum) { mine[b] = sum; });
+    rank_tile(d, digit.bits, buckets, warp_counts, rank, [&](uint32_t b, uint32_t sum) { mine[b] = sum; });
 #pragma unroll
     for (uint32_t r = 0; r < kRounds; r++) {
         const uint32_t i = first + tile_item(r);
@@ -323,13 +378,16 @@ __global__ void __launch_bounds__(1024) bucket_scan_kernel(uint32_t *__restrict_
     const uint32_t b = blockIdx.x * 32 + x;
     const uint32_t each = (tiles + 31) / 32, t0 = min(y * each, tiles), t1 = min(t0 + each, tiles);
     uint32_t sum = 0;
-    if (b < buckets)
+    if (b < buckets) {
+#pragma unroll 8
         for (uint32_t t = t0; t < t1; t++) sum += counts[(uint64_t) t * buckets + b];
+    }
     part[y][x] = sum;
     __syncthreads();
     uint32_t run = 0;
     for (uint32_t i = 0; i < y; i++) run += part[i][x];
     if (b < buckets) {
+#pragma unroll 8
         for (uint32_t t = t0; t < t1; t++) {
             const uint32_t c = counts[(uint64_t) t * buckets + b];
             counts[(uint64_t) t * buckets + b] = run;
@@ -340,81 +398,69 @@ __global__ void __launch_bounds__(1024) bucket_scan_kernel(uint32_t *__restrict_
 }
 
 template<typename To, bool kScanned>
-__global__ void __launch_bounds__(1024) bucket_place_kernel(const uint32_t *__restrict__ keys, uint32_t items, Digit digit, uint32_t buckets,
-                                                            const uint32_t *__restrict__ counts, uint32_t tiles, const uint32_t *__restrict__ totals,
-                                                            const uint16_t *__restrict__ ranks, To to) {
-    extern __shared__ __align__(16) uint32_t base[];   // of each bucket: all items of smaller ones, then the tiles before, too
+__global__ void __launch_bounds__(kTileThreads) bucket_place_kernel(Keys keys, uint32_t items, Digit digit, uint32_t buckets, uint32_t tiles,
+                                                                    const uint32_t *__restrict__ counts, const uint32_t *__restrict__ totals,
+                                                                    const uint16_t *__restrict__ ranks, To to, Clear clear) {
+    extern __shared__ __align__(16) uint32_t base[];   // of each bucket: all items of smaller ones; then, behind, its items in the tiles before
+    if (blockIdx.x >= tiles) return clear.block(blockIdx.x - tiles);
     wait_for_previous();
-    const uint32_t first = blockIdx.x * (blockDim.x * kRounds);
-    uint32_t key[kRounds], rank[kRounds], value[kRounds];
+    uint32_t *before = base + buckets;
+    const uint32_t first = blockIdx.x * kTile;
+    uint2 item[kRounds];
+    uint32_t rank[kRounds];
 #pragma unroll
     for (uint32_t r = 0; r < kRounds; r++) {
-        const uint32_t i = min(first + r * blockDim.x + threadIdx.x, items - 1);
-        key[r] = min(keys[i], digit.limit);
+        const uint32_t i = min(first + r * kTileThreads + threadIdx.x, items - 1);
+        item[r] = keys.item(i);
         rank[r] = ranks[i];
-        value[r] = to.value_of(i);
     }
-    uint32_t before[(kMaxPartitions + 1 + 511) / 512];   // the launcher gives a thread no more buckets than that
-    uint32_t n = 0;
-#pragma unroll
-    for (uint32_t q = 0; q < sizeof before / sizeof *before; q++) {
-        const uint32_t b = q * blockDim.x + threadIdx.x;
-        if (b >= buckets) break;
+    for (uint32_t b = threadIdx.x; b < buckets; b += kTileThreads) {
         uint32_t all = 0, mine = 0;
         if constexpr (kScanned) {
             all = totals[b];
             mine = counts[(uint64_t) blockIdx.x * buckets + b];
         } else {
-#pragma unroll 8
+#pragma unroll 16
             for (uint32_t t = 0; t < tiles; t++) {
-                const uint32_t c = counts[(uint64_t) t * buckets + b];
+                const uint32_t c = counts[t * buckets + b];
                 mine += t < blockIdx.x ? c : 0;
                 all += c;
             }
         }
         base[b] = all;
-        before[q] = mine;
-        n = q + 1;
+        before[b] = mine;
     }
     scan_buckets(base, buckets);
-#pragma unroll
-    for (uint32_t q = 0; q < sizeof before / sizeof *before; q++) {
-        if (q >= n) break;
-        const uint32_t b = q * blockDim.x + threadIdx.x;
-        if (blockIdx.x == 0) to.start(b, base[b]);
-        base[b] += before[q];
-    }
-    __syncthreads();
+    if (blockIdx.x == 0)
+        for (uint32_t b = threadIdx.x; b < buckets; b += kTileThreads) to.start(b, base[b]);
 #pragma unroll
     for (uint32_t r = 0; r < kRounds; r++) {
-        const uint32_t i = first + r * blockDim.x + threadIdx.x;
-        if (i < items) to.item(i, value[r], key[r], digit, base[digit.of(key[r])] + rank[r]);
+        const uint32_t d = digit.of(item[r].x);
+        if (first + r * kTileThreads + threadIdx.x < items) to.item(item[r], digit, base[d] + before[d] + rank[r]);
     }
 }
 
 // One tile: ranks and places in one launch.
 template<typename To>
-__device__ __forceinline__ void sort_tile(const uint32_t *keys, uint32_t items, const Digit &digit, uint32_t buckets, uint32_t *base, uint16_t *warp_counts, const To &to) {
-    uint32_t key[kRounds], d[kRounds], rank[kRounds], value[kRounds];
+__device__ __forceinline__ void sort_tile(const Keys &keys, uint32_t items, const Digit &digit, uint32_t buckets, uint32_t *base, uint16_t *warp_counts, const To &to) {
+    uint2 item[kRounds];
+    uint32_t d[kRounds], rank[kRounds];
 #pragma unroll
     for (uint32_t r = 0; r < kRounds; r++) {
         const uint32_t i = tile_item(r);
-        key[r] = i < items ? min(keys[i], digit.limit) : kNone;
-        d[r] = i < items ? digit.of(key[r]) : kNone;
-        value[r] = i < items ? to.value_of(i) : 0;
+        item[r] = keys.item(min(i, items - 1));
+        d[r] = i < items ? digit.of(item[r].x) : kNone;
     }
-    rank_tile(d, buckets, warp_counts, rank, [&](uint32_t b, uint32_t sum) { base[b] = sum; });
+    rank_tile(d, digit.bits, buckets, warp_counts, rank, [&](uint32_t b, uint32_t sum) { base[b] = sum; });
     scan_buckets(base, buckets);
     for (uint32_t b = threadIdx.x; b < buckets; b += blockDim.x) to.start(b, base[b]);
 #pragma unroll
-    for (uint32_t r = 0; r < kRounds; r++) {
-        const uint32_t i = tile_item(r);
-        if (i < items) to.item(i, value[r], key[r], digit, base[d[r]] + rank[r]);
-    }
+    for (uint32_t r = 0; r < kRounds; r++)
+        if (d[r] != kNone) to.item(item[r], digit, base[d[r]] + rank[r]);
     __syncthreads();
 }
 
-__global__ void __launch_bounds__(1024) place_tile_kernel(const uint32_t *keys, uint32_t items, Digit digit, uint32_t buckets, ToPlaces to) {
+__global__ void __launch_bounds__(kOneTile / kRounds) place_tile_kernel(Keys keys, uint32_t items, Digit digit, uint32_t buckets, ToPlaces to) {
     extern __shared__ __align__(16) uint16_t warp_counts[];
     uint32_t *base = reinterpret_cast<uint32_t *>(reinterpret_cast<char *>(warp_counts) + rank_smem(blockDim.x >> 5, buckets));
     wait_for_previous();
@@ -422,30 +468,31 @@ __global__ void __launch_bounds__(1024) place_tile_kernel(const uint32_t *keys, 
 }
 
 // All passes of a radix sort of one tile; the items lie in global memory between passes (the CTA's barriers order them).
-__global__ void __launch_bounds__(1024) sort_tile_kernel(const uint32_t *keys, uint32_t items, uint32_t limit, uint32_t bits, uint32_t pass_bits,
-                                                         uint32_t *keys0, uint32_t *values0, uint32_t *keys1, uint32_t *values1) {
+__global__ void __launch_bounds__(kOneTile / kRounds) sort_tile_kernel(const uint32_t *keys, uint32_t items, uint32_t limit, uint32_t bits, uint32_t pass_bits,
+                                                                       uint2 *items0, uint2 *items1, Clear clear) {
     extern __shared__ __align__(16) uint16_t warp_counts[];
     uint32_t *base = reinterpret_cast<uint32_t *>(reinterpret_cast<char *>(warp_counts) + rank_smem(blockDim.x >> 5, 1u << pass_bits));
+    if (blockIdx.x >= 1) return clear.block(blockIdx.x - 1);
     wait_for_previous();
-    const uint32_t *in = keys, *values = nullptr;
+    Keys in{keys, nullptr};
     for (uint32_t shift = 0, pass = 0; shift < bits; shift += pass_bits, pass++) {
-        uint32_t *k = pass & 1 ? keys1 : keys0, *v = pass & 1 ? values1 : values0;
+        uint2 *to = pass & 1 ? items1 : items0;
         const uint32_t here = min(pass_bits, bits - shift);
-        sort_tile(in, items, Digit{limit, shift, (1u << here) - 1}, 1u << here, base, warp_counts, ToSorted{values, k, v});
-        in = k;
-        values = v;
+        sort_tile(in, items, Digit{limit, shift, here}, 1u << here, base, warp_counts, ToSorted{to});
+        in = Keys{nullptr, to};
     }
 }
 
 // ---- gradient of a lookup ---------------------------------------------------------------------------------------
 struct GradArgs {
-    const uint32_t *keys, *values;   // sorted by id: the id, and the row of grad_out
+    const uint2 *sorted;             // by id: the id, and the row of the gradient
     uint32_t items, n, dim, words, lanes, slabs, chunk;
     float scale;
     uint64_t in_stride, out_stride;
     int accumulate;
     float *partial;                  // (2 * chunk + which) * dim: sums of runs that leave their chunk
-    uint32_t join_blocks, zero_rows; // CTAs that join; the others clear zero_rows rows each
+    uint32_t join_blocks, clear_from, clear_rows;   // CTAs that join; the others clear clear_rows rows each, from row clear_from on
+    __device__ __forceinline__ uint32_t key(uint64_t i) const { return sorted[i].x; }
 };
 
 template<typename O, int V>
@@ -463,11 +510,11 @@ __device__ __forceinline__ void put_grad(O *out, const GradArgs &a, uint32_t id,
 }
 
 // The first of the sorted keys from `lo` on that is not below `key`; the CTA narrows the range by its width at each step.
-__device__ __forceinline__ uint32_t first_not_below(const uint32_t *__restrict__ keys, uint32_t lo, uint32_t hi, uint32_t key) {
+__device__ __forceinline__ uint32_t first_not_below(const uint2 *__restrict__ sorted, uint32_t lo, uint32_t hi, uint32_t key) {
     while (lo < hi) {
         const uint32_t step = (hi - lo + blockDim.x - 1) / blockDim.x;
         const uint64_t i = lo + (uint64_t) threadIdx.x * step;
-        const uint32_t below = __syncthreads_count(i < hi && keys[i] < key);
+        const uint32_t below = __syncthreads_count(i < hi && sorted[i].x < key);
         if (below == 0) break;
         const uint64_t end = lo + (uint64_t) below * step;
         lo += (below - 1) * step + 1;
@@ -482,15 +529,15 @@ __device__ __forceinline__ void clear_rows(O *out, const GradArgs &a, uint32_t r
     __shared__ uint32_t named[256 / 32];   // a CTA clears 256 rows at most
     if (threadIdx.x < 8) named[threadIdx.x] = 0;
     __syncthreads();
-    uint32_t at = first_not_below(a.keys, 0, a.items, r0);
+    uint32_t at = first_not_below(a.sorted, 0, a.items, r0);
     while (at < a.items) {
-        const uint32_t i = at + threadIdx.x, key = i < a.items ? a.keys[i] : kNone;
+        const uint32_t i = at + threadIdx.x, key = i < a.items ? a.key(i) : kNone;
         if (key < r1) atomicOr(&named[(key - r0) >> 5], 1u << ((key - r0) & 31u));
         const uint32_t here = __syncthreads_count(key < r1);
         if (here < blockDim.x) break;
         // a whole CTA's width of one id: on to the next id
-        const uint32_t head = a.keys[at];
-        at = a.keys[at + blockDim.x - 1] == head ? first_not_below(a.keys, at + blockDim.x, a.items, head + 1) : at + blockDim.x;
+        const uint32_t head = a.key(at);
+        at = a.key(at + blockDim.x - 1) == head ? first_not_below(a.sorted, at + blockDim.x, a.items, head + 1) : at + blockDim.x;
     }
     __syncthreads();
     float zero[V];
@@ -509,8 +556,8 @@ __global__ void __launch_bounds__(256) grad_join_kernel(const T *__restrict__ gr
     constexpr int U = 8;
     wait_for_previous();
     if (blockIdx.x >= a.join_blocks) {
-        const uint64_t r0 = (uint64_t) (blockIdx.x - a.join_blocks) * a.zero_rows;
-        clear_rows<O, V>(out, a, (uint32_t) r0, (uint32_t) min((uint64_t) a.n, r0 + a.zero_rows));
+        const uint64_t r0 = a.clear_from + (uint64_t) (blockIdx.x - a.join_blocks) * a.clear_rows;
+        clear_rows<O, V>(out, a, (uint32_t) r0, (uint32_t) min((uint64_t) a.n, r0 + a.clear_rows));
         return;
     }
     const uint32_t group = (blockIdx.x * 256 + threadIdx.x) / a.lanes, lane = threadIdx.x & (a.lanes - 1);
@@ -518,8 +565,8 @@ __global__ void __launch_bounds__(256) grad_join_kernel(const T *__restrict__ gr
     const uint64_t c0 = (uint64_t) chunk * a.chunk;
     if (c0 >= a.items || word >= a.words) return;
     const uint32_t c1 = (uint32_t) min(c0 + a.chunk, (uint64_t) a.items), at = word * V;
-    uint32_t id = a.keys[c0];
-    bool from_left = c0 > 0 && a.keys[c0 - 1] == id;
+    uint32_t id = a.key(c0);
+    bool from_left = c0 > 0 && a.key(c0 - 1) == id;
     float acc[V];
 #pragma unroll
     for (int i = 0; i < V; i++) acc[i] = 0.0f;
@@ -533,9 +580,9 @@ __global__ void __launch_bounds__(256) grad_join_kernel(const T *__restrict__ gr
         WordOf<T, V> w[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const uint32_t i = min(c + u, c1 - 1);
-            key[u] = a.keys[i];
-            value[u] = a.values[i];
+            const uint2 item = __ldg(a.sorted + min(c + u, c1 - 1));
+            key[u] = item.x;
+            value[u] = item.y;
         }
 #pragma unroll
         for (int u = 0; u < U; u++) w[u] = get_word_if<WordOf<T, V>>(grad + (uint64_t) value[u] * a.in_stride + at, key[u] < a.n);
@@ -557,47 +604,79 @@ __global__ void __launch_bounds__(256) grad_join_kernel(const T *__restrict__ gr
             }
         }
     }
-    put(c1 < a.items && a.keys[c1] == id);
+    put(c1 < a.items && a.key(c1) == id);
 }
 
-// Runs over several chunks: the CTA of the chunk that a run starts in adds its partial sums. Each of its eight warps takes an eighth of
-// the run's chunks, in order, and the warps' sums are added in order: the shape of the sum depends on the run alone.
+// Runs over several chunks, whose first chunk's unit (a chunk and a slab) adds their partial sums and writes the row. A warp owns a unit and
+// adds short runs by itself, in order; of a run with more partial sums than kLongRun each of the CTA's eight warps takes an
+// eighth, in order, and their sums are added in order. The shape of a sum depends on the run alone.
+constexpr uint32_t kLongRun = 32;
 template<typename O, int V>
-__global__ void __launch_bounds__(256) grad_fix_kernel(O *__restrict__ out, GradArgs a) {
+__global__ void __launch_bounds__(256) grad_fix_kernel(O *__restrict__ out, GradArgs a, uint32_t units) {
     __shared__ float part[8][32][V];
+    __shared__ uint32_t long_last[8];
     wait_for_previous();
-    const uint32_t chunk = blockIdx.x / a.slabs, slab = blockIdx.x - chunk * a.slabs;
-    const uint64_t c0 = (uint64_t) chunk * a.chunk, c1 = c0 + a.chunk;
-    if (c1 >= a.items) return;
-    const uint32_t id = a.keys[c1 - 1];
-    if (id >= a.n || a.keys[c1] != id || (a.keys[c0] == id && c0 > 0 && a.keys[c0 - 1] == id)) return;
-    // the run's last chunk; the whole CTA is here
-    const uint32_t end = first_not_below(a.keys, (uint32_t) c1, a.items, id + 1), last = (end - 1) / a.chunk;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-    const uint32_t word = slab * a.lanes + (lane & (a.lanes - 1)), at = word * V;
-    const bool mine = lane < a.lanes && word < a.words;
-    const uint32_t sums = last - chunk + 1, each = (sums + 7) / 8, s0 = min(warp * each, sums), s1 = min(s0 + each, sums);
-    float acc[V];
+    auto add = [&](uint32_t chunk, uint32_t at, uint32_t s0, uint32_t s1, float (&acc)[V]) {   // partial sums s0 .. s1 - 1 of the run that starts in chunk
 #pragma unroll
-    for (int i = 0; i < V; i++) acc[i] = 0.0f;
-    if (mine) {
-#pragma unroll 4
+        for (int i = 0; i < V; i++) acc[i] = 0.0f;
+#pragma unroll 8
         for (uint32_t s = s0; s < s1; s++) {
             float f[V];
             load<float, V>(a.partial + (2ull * (chunk + s) + (s == 0 ? 1 : 0)) * a.dim + at, f);
 #pragma unroll
             for (int i = 0; i < V; i++) acc[i] += f[i];
         }
-#pragma unroll
-        for (int i = 0; i < V; i++) part[warp][lane][i] = acc[i];
+    };
+    const uint32_t unit = blockIdx.x * 8 + warp;
+    uint32_t last = 0;   // the run's last chunk; 0: no run starts here and goes on
+    if (unit < units) {
+        const uint32_t chunk = unit / a.slabs, word = (unit - chunk * a.slabs) * a.lanes + lane;
+        const uint64_t c0 = (uint64_t) chunk * a.chunk, c1 = c0 + a.chunk;   // below a.items, as the last chunk has no unit
+        const uint32_t id = a.key(c1 - 1);
+        if (id < a.n && a.key(c1) == id && !(a.key(c0) == id && c0 > 0 && a.key(c0 - 1) == id)) {
+            // the first chunk boundary that the run does not cross, among the next 32 at a time
+            uint32_t c = chunk + 1;
+            while (true) {
+                const uint64_t end = (uint64_t) (c + lane + 1) * a.chunk;
+                const uint32_t beyond = __ballot_sync(0xffffffffu, end >= a.items || a.key(end < a.items ? end : 0) != id);
+                if (beyond) {
+                    last = c + __ffs(beyond) - 1;
+                    break;
+                }
+                c += 32;
+            }
+            if (last - chunk < kLongRun && lane < a.lanes && word < a.words) {
+                float acc[V];
+                add(chunk, word * V, 0, last - chunk + 1, acc);
+                put_grad<O, V>(out, a, id, word * V, acc);
+            }
+            if (last - chunk < kLongRun) last = 0;
+        }
     }
-    __syncthreads();
-    if (warp != 0 || !mine) return;
+    if (lane == 0) long_last[warp] = last;
+    if (!__syncthreads_or(last)) return;
+    for (uint32_t u = 0; u < 8; u++) {
+        if (long_last[u] == 0) continue;
+        const uint32_t chunk = (blockIdx.x * 8 + u) / a.slabs, word = (blockIdx.x * 8 + u - chunk * a.slabs) * a.lanes + lane;
+        const uint32_t sums = long_last[u] - chunk + 1, each = (sums + 7) / 8, s0 = min(warp * each, sums), s1 = min(s0 + each, sums);
+        const bool mine = lane < a.lanes && word < a.words;
+        float acc[V];
+        if (mine) {
+            add(chunk, word * V, s0, s1, acc);
 #pragma unroll
-    for (int w = 1; w < 8; w++)
+            for (int i = 0; i < V; i++) part[warp][lane][i] = acc[i];
+        }
+        __syncthreads();
+        if (warp == 0 && mine) {
 #pragma unroll
-        for (int i = 0; i < V; i++) acc[i] += part[w][lane][i];
-    put_grad<O, V>(out, a, id, at, acc);
+            for (int w = 1; w < 8; w++)
+#pragma unroll
+                for (int i = 0; i < V; i++) acc[i] += part[w][lane][i];
+            put_grad<O, V>(out, a, a.key((uint64_t) (chunk + 1) * a.chunk - 1), word * V, acc);
+        }
+        __syncthreads();
+    }
 }
 
 // ---- dispatch ---------------------------------------------------------------------------------------------------
@@ -882,53 +961,55 @@ cudaError_t launch_lookup(const void *table, uint64_t table_stride, uint32_t n, 
     return cudaSuccess;
 }
 
-// The shape of a counting sort: 1,024 threads a CTA, 512 where the counters of 32 warps would not fit.
-struct Tiles {
-    uint32_t threads, items, count;
-    Tiles(uint64_t all, uint32_t buckets) : threads(buckets > (1u << kMaxPassBits) ? 512 : 1024), items(threads * kRounds), count((uint32_t) ceil_div(all, items)) {}
-};
+uint32_t bits_for(uint64_t values) {   // to write 0 .. values - 1
+    uint32_t bits = 1;
+    while ((1ull << bits) < values) bits++;
+    return bits;
+}
 
-// One pass over more than one tile.
-template<typename To>
-cudaError_t sort_pass(const uint32_t *keys, uint32_t items, const Digit &digit, uint32_t buckets, uint32_t *counts, uint32_t *totals, uint16_t *ranks,
-                      const To &to, bool dependent, cudaStream_t stream) {
-    const Tiles t(items, buckets);
-    cudaError_t e = launch(bucket_count_kernel, t.count, t.threads, rank_smem(t.threads / 32, buckets), stream, dependent, keys, items, digit, buckets, counts, ranks);
+// One pass over more than one tile; `clear` gives the next rows to clear to each launch that has room for it.
+template<typename To, typename C>
+cudaError_t sort_pass(const Keys &keys, uint32_t items, const Digit &digit, uint32_t buckets, uint32_t *counts, uint32_t *totals, uint16_t *ranks,
+                      const To &to, bool dependent, cudaStream_t stream, C clear) {
+    const uint32_t tiles = (uint32_t) ceil_div(items, kTile);
+    Clear c = clear();
+    cudaError_t e = launch(bucket_count_kernel, tiles + c.blocks(), kTileThreads, rank_smem(kTileThreads / 32, buckets), stream, dependent, keys, items, digit, buckets, tiles, counts, ranks, c);
     if (e != cudaSuccess) return e;
-    if (t.count <= kMaxFusedTiles)
-        return launch(bucket_place_kernel<To, false>, t.count, t.threads, buckets * 4, stream, true, keys, items, digit, buckets, counts, t.count, totals, ranks, to);
-    e = launch(bucket_scan_kernel, ceil_div(buckets, 32), 1024, 0, stream, true, counts, t.count, buckets, totals);
+    c = clear();
+    if (tiles <= kMaxFusedTiles)
+        return launch(bucket_place_kernel<To, false>, tiles + c.blocks(), kTileThreads, buckets * 8, stream, true, keys, items, digit, buckets, tiles, counts, totals, ranks, to, c);
+    e = launch(bucket_scan_kernel, ceil_div(buckets, 32), 1024, 0, stream, true, counts, tiles, buckets, totals);
     if (e != cudaSuccess) return e;
-    return launch(bucket_place_kernel<To, true>, t.count, t.threads, buckets * 4, stream, true, keys, items, digit, buckets, counts, t.count, totals, ranks, to);
+    return launch(bucket_place_kernel<To, true>, tiles + c.blocks(), kTileThreads, buckets * 8, stream, true, keys, items, digit, buckets, tiles, counts, totals, ranks, to, c);
 }
 
 // Scratch of the gradient: two copies of the sorted items, the counts of a pass, the partial sums of its chunks.
 struct GradScratch {
-    uint32_t *keys[2], *values[2], *counts, *totals;
+    uint2 *items[2];
+    uint32_t *counts, *totals;
     uint16_t *ranks;
     float *partial;
     uint32_t bits, passes, pass_bits, chunk;
     uint64_t bytes;
-    GradScratch(void *base, uint64_t n, uint64_t items, uint32_t dim) {
-        bits = 1;
-        while ((1ull << bits) <= n) bits++;             // ids 0 .. n - 1, and n for none
+    GradScratch(void *base, uint64_t n, uint64_t count, uint32_t dim) {
+        bits = bits_for(n + 1);             // ids 0 .. n - 1, and n for none
         passes = (bits + kMaxPassBits - 1) / kMaxPassBits;
         pass_bits = (bits + passes - 1) / passes;
+        // Long chunks leave few partial sums, short ones many groups of lanes to work: as long as some 32 warps an SM remain
+        // (counted for words of 16 bytes of bf16).
         chunk = 32;
+        while (chunk < 128 && count * ceil_div(dim, 256) / chunk >= 2 * 148 * 32) chunk *= 2;
         uint64_t at = 0;
         auto take = [&](uint64_t size) {
             const uint64_t here = at;
             at += align256(size);
             return static_cast<char *>(base) + here;
         };
-        for (int i = 0; i < 2; i++) {
-            keys[i] = reinterpret_cast<uint32_t *>(take(items * 4));
-            values[i] = reinterpret_cast<uint32_t *>(take(items * 4));
-        }
-        ranks = reinterpret_cast<uint16_t *>(take(items * 2));
-        counts = reinterpret_cast<uint32_t *>(take(((uint64_t) Tiles(items, 1u << pass_bits).count << pass_bits) * 4));
+        for (int i = 0; i < 2; i++) items[i] = reinterpret_cast<uint2 *>(take(count * 8));
+        ranks = reinterpret_cast<uint16_t *>(take(count * 2));
+        counts = reinterpret_cast<uint32_t *>(take((ceil_div(count, kTile) << pass_bits) * 4));
         totals = reinterpret_cast<uint32_t *>(take(4ull << pass_bits));
-        partial = reinterpret_cast<float *>(take(2 * ceil_div(items, chunk) * dim * 4));
+        partial = reinterpret_cast<float *>(take(2 * ceil_div(count, chunk) * dim * 4));
         bytes = at;
     }
 };
@@ -938,15 +1019,14 @@ struct DispatchScratch {
     uint16_t *ranks = nullptr;
     uint64_t bytes = 0;
     DispatchScratch(void *base, uint64_t pairs, uint32_t partitions) {
-        const Tiles t(pairs, partitions + 1);
-        if (pairs <= kSmallPairs || t.count <= 1) return;
+        if (pairs <= kOneTile) return;
         auto take = [&](uint64_t size) {
             const uint64_t here = bytes;
             bytes += align256(size);
             return static_cast<char *>(base) + here;
         };
         ranks = reinterpret_cast<uint16_t *>(take(pairs * 2));
-        counts = reinterpret_cast<uint32_t *>(take((uint64_t) t.count * (partitions + 1) * 4));
+        counts = reinterpret_cast<uint32_t *>(take(ceil_div(pairs, kTile) * (partitions + 1) * 4));
         totals = reinterpret_cast<uint32_t *>(take((partitions + 1) * 4ull));
     }
 };
@@ -1008,31 +1088,41 @@ int glide_lookup_rows_grad(glide_ctx *ctx, const void *d_grad, int row_type, uin
     ROWS_CUDA(guard.status);
     auto s = static_cast<cudaStream_t>(stream);
     const GradScratch w(d_workspace, n, count, dim);
-    const uint32_t items = (uint32_t) count;
-    const uint32_t *keys = d_ids, *values = nullptr;
-    if (count > 0 && Tiles(items, 1u << w.pass_bits).count == 1) {
-        const uint32_t threads = (uint32_t) ceil_div(items, kRounds * 32) * 32, last = (w.passes - 1) & 1;
-        ROWS_CUDA(launch(sort_tile_kernel, 1, threads, rank_smem(threads / 32, 1u << w.pass_bits) + (4u << w.pass_bits), s, false, d_ids, items, (uint32_t) n, w.bits, w.pass_bits,
-                         w.keys[0], w.values[0], w.keys[1], w.values[1]));
-        keys = w.keys[last];
-        values = w.values[last];
+    const uint32_t items = (uint32_t) count, row_bytes = dim * bytes_of(grad_type);
+    // Rows are cleared where the memory is idle: a share with each launch of the sort, whether an id names them or not, as long as ids are
+    // few beside rows; the rest by the kernel that joins, which by then knows the rows that no id names.
+    uint32_t clear_each = (128u << 10) / row_bytes, cleared = 0;   // a CTA clears up to 128 KB
+    clear_each = clear_each < 1 ? 1 : clear_each > 256 ? 256 : clear_each;
+    const uint64_t share = accumulate || count >= n / 2 ? 0 : kClearShare / row_bytes;
+    auto clear = [&]() {
+        Clear c{static_cast<uint8_t *>(d_table_grad) + (uint64_t) cleared * table_grad_stride * bytes_of(grad_type), table_grad_stride * bytes_of(grad_type), row_bytes,
+                (uint32_t) (share < n - cleared ? share : n - cleared), clear_each, 2};
+        const uint64_t any = reinterpret_cast<uintptr_t>(c.at) | c.stride | c.bytes;
+        c.word = any % 16 == 0 ? 16 : any % 4 == 0 ? 4 : 2;
+        cleared += c.rows;
+        return c;
+    };
+    const uint2 *sorted = nullptr;
+    if (count > 0 && count <= kOneTile) {
+        const uint32_t threads = (uint32_t) ceil_div(items, kRounds * 32) * 32;
+        const Clear c = clear();
+        ROWS_CUDA(launch(sort_tile_kernel, 1 + c.blocks(), threads, rank_smem(threads / 32, 1u << w.pass_bits) + (4u << w.pass_bits), s, false, d_ids, items, (uint32_t) n, w.bits, w.pass_bits,
+                         w.items[0], w.items[1], c));
+        sorted = w.items[(w.passes - 1) & 1];
     } else if (count > 0) {
         for (uint32_t pass = 0; pass < w.passes; pass++) {
-            const uint32_t left = w.bits - pass * w.pass_bits, here = left < w.pass_bits ? left : w.pass_bits, buckets = 1u << here;
-            ROWS_CUDA(sort_pass(keys, items, Digit{(uint32_t) n, pass * w.pass_bits, buckets - 1}, buckets, w.counts, w.totals, w.ranks, ToSorted{values, w.keys[pass & 1], w.values[pass & 1]}, pass > 0, s));
-            keys = w.keys[pass & 1];
-            values = w.values[pass & 1];
+            const uint32_t left = w.bits - pass * w.pass_bits, here = left < w.pass_bits ? left : w.pass_bits;
+            ROWS_CUDA(sort_pass(Keys{d_ids, sorted}, items, Digit{(uint32_t) n, pass * w.pass_bits, here}, 1u << here, w.counts, w.totals, w.ranks, ToSorted{w.items[pass & 1]}, pass > 0, s, clear));
+            sorted = w.items[pass & 1];
         }
     }
     const uint32_t most = most_of(row_type), v0 = count ? in.width(most) : most, v1 = out.width(most), v = v0 < v1 ? v0 : v1;
-    GradArgs a{keys, values, items, (uint32_t) n, dim, dim / v, 32, 1, w.chunk, scale, grad_stride, table_grad_stride, accumulate, w.partial, 0, 0};
+    GradArgs a{sorted, items, (uint32_t) n, dim, dim / v, 32, 1, w.chunk, scale, grad_stride, table_grad_stride, accumulate, w.partial, 0, cleared, clear_each};
     while (a.lanes > 1 && a.lanes / 2 >= a.words) a.lanes /= 2;
     a.slabs = (uint32_t) ceil_div(a.words, a.lanes);
-    const uint64_t chunks = ceil_div(items, a.chunk), join = ceil_div(chunks * a.slabs * a.lanes, 256);
-    a.zero_rows = (128u << 10) / (dim * bytes_of(grad_type));   // a CTA clears up to 128 KB
-    a.zero_rows = a.zero_rows < 1 ? 1 : a.zero_rows > 256 ? 256 : a.zero_rows;
-    const uint64_t zero = accumulate ? 0 : ceil_div(n, a.zero_rows);
-    ROWS_REQUIRE(join <= 0xffffffu && chunks * a.slabs <= 0x7fffffffu && join + zero <= 0x7fffffffu, GLIDE_ERR_UNSUPPORTED, "lookup_rows_grad: too many values in one call");   // threads are counted in 32 bits
+    const uint64_t chunks = ceil_div(items, a.chunk), join = ceil_div(chunks * a.slabs * a.lanes, 256), units = chunks < 2 ? 0 : (chunks - 1) * a.slabs;
+    const uint64_t zero = accumulate ? 0 : ceil_div(n - cleared, clear_each);
+    ROWS_REQUIRE(join <= 0xffffffu && units <= 0x7fffffffu && join + zero <= 0x7fffffffu, GLIDE_ERR_UNSUPPORTED, "lookup_rows_grad: too many values in one call");   // threads are counted in 32 bits
     a.join_blocks = (uint32_t) join;
     if (join + zero == 0) return GLIDE_OK;
     auto run = [&](auto t, auto o, auto wd) {
@@ -1040,8 +1130,8 @@ int glide_lookup_rows_grad(glide_ctx *ctx, const void *d_grad, int row_type, uin
         using O = decltype(o);
         constexpr int V = decltype(wd)::value;
         const cudaError_t e = launch(grad_join_kernel<T, O, V>, join + zero, 256, 0, s, count > 0, static_cast<const T *>(d_grad), static_cast<O *>(d_table_grad), a);
-        if (e != cudaSuccess || chunks < 2) return e;
-        return launch(grad_fix_kernel<O, V>, (chunks - 1) * a.slabs, 256, 0, s, true, static_cast<O *>(d_table_grad), a);
+        if (e != cudaSuccess || units == 0) return e;
+        return launch(grad_fix_kernel<O, V>, ceil_div(units, 8), 256, 0, s, true, static_cast<O *>(d_table_grad), a, (uint32_t) units);
     };
     ROWS_CUDA(with_rows(row_type, v, [&](auto t, auto wd) { return grad_type == GLIDE_ROW_F32 ? run(t, float{}, wd) : run(t, t, wd); }));
     return GLIDE_OK;
@@ -1100,14 +1190,13 @@ int glide_dispatch_rows(glide_ctx *ctx, const void *d_rows, int row_type, uint64
         return GLIDE_OK;
     }
     const DispatchScratch w(d_workspace, pairs, partitions);
-    const Tiles tiles(pairs, partitions + 1);
-    const Digit digit{partitions, 0, kNone};
+    const Digit digit{partitions, 0, bits_for(partitions + 1)};
     const ToPlaces places{d_position, d_map, d_segment_start, Div(choices)};
-    if (tiles.count == 1) {
+    if (pairs <= kOneTile) {
         const uint32_t threads = (uint32_t) ceil_div(pairs, kRounds * 32) * 32;
-        ROWS_CUDA(launch(place_tile_kernel, 1, threads, rank_smem(threads / 32, partitions + 1) + (partitions + 1) * 4, s, false, d_choice, (uint32_t) pairs, digit, partitions + 1, places));
+        ROWS_CUDA(launch(place_tile_kernel, 1, threads, rank_smem(threads / 32, partitions + 1) + (partitions + 1) * 4, s, false, Keys{d_choice, nullptr}, (uint32_t) pairs, digit, partitions + 1, places));
     } else {
-        ROWS_CUDA(sort_pass(d_choice, (uint32_t) pairs, digit, partitions + 1, w.counts, w.totals, w.ranks, places, false, s));
+        ROWS_CUDA(sort_pass(Keys{d_choice, nullptr}, (uint32_t) pairs, digit, partitions + 1, w.counts, w.totals, w.ranks, places, false, s, [] { return Clear{}; }));
     }
     const uint64_t each = 0x7fff0000u / words;   // rows of a launch: its words are counted in 31 bits
     for (uint64_t r0 = 0; r0 < count; r0 += each) {
