@@ -281,6 +281,8 @@ __device__ __forceinline__ void rank_tile(const uint32_t (&d)[kRounds], uint32_t
         if (d[r] != kNone) rank[r] += mine[d[r]];
 }
 
+// Counts of a tile lie in whole words of four.
+__host__ __device__ constexpr uint32_t count_stride(uint32_t buckets) { return (buckets + 3) & ~3u; }
 __host__ __device__ constexpr uint32_t rank_smem(uint32_t warps, uint32_t buckets) { return (warps * buckets + 7) / 8 * 16; }
 
 // Exclusive sums over `buckets` values, in place in shared memory, which the CTA has written.
@@ -360,7 +362,9 @@ __global__ void __launch_bounds__(kTileThreads) bucket_count_kernel(Keys keys, u
         const uint32_t i = first + tile_item(r);
         d[r] = i < items ? digit.of(keys.key(i)) : kNone;
     }
-    uint32_t *mine = counts + (uint64_t) blockIdx.x * buckets;
+    const uint32_t stride = count_stride(buckets);
+    uint32_t *mine = counts + (uint64_t) blockIdx.x * stride;
+    if (threadIdx.x < stride - buckets) mine[buckets + threadIdx.x] = 0;
     rank_tile(d, digit.bits, buckets, warp_counts, rank, [&](uint32_t b, uint32_t sum) { mine[b] = sum; });
 #pragma unroll
     for (uint32_t r = 0; r < kRounds; r++) {
@@ -374,13 +378,14 @@ __global__ void __launch_bounds__(1024) bucket_scan_kernel(uint32_t *__restrict_
                                                            uint32_t *__restrict__ totals) {
     __shared__ uint32_t part[32][33];
     wait_for_previous();
+    const uint32_t stride = count_stride(buckets);
     const uint32_t x = threadIdx.x & 31u, y = threadIdx.x >> 5;
     const uint32_t b = blockIdx.x * 32 + x;
     const uint32_t each = (tiles + 31) / 32, t0 = min(y * each, tiles), t1 = min(t0 + each, tiles);
     uint32_t sum = 0;
     if (b < buckets) {
 #pragma unroll 8
-        for (uint32_t t = t0; t < t1; t++) sum += counts[(uint64_t) t * buckets + b];
+        for (uint32_t t = t0; t < t1; t++) sum += counts[(uint64_t) t * stride + b];
     }
     part[y][x] = sum;
     __syncthreads();
@@ -389,8 +394,8 @@ __global__ void __launch_bounds__(1024) bucket_scan_kernel(uint32_t *__restrict_
     if (b < buckets) {
 #pragma unroll 8
         for (uint32_t t = t0; t < t1; t++) {
-            const uint32_t c = counts[(uint64_t) t * buckets + b];
-            counts[(uint64_t) t * buckets + b] = run;
+            const uint32_t c = counts[(uint64_t) t * stride + b];
+            counts[(uint64_t) t * stride + b] = run;
             run += c;
         }
         if (y == 31) totals[b] = run;
@@ -404,7 +409,8 @@ __global__ void __launch_bounds__(kTileThreads) bucket_place_kernel(Keys keys, u
     extern __shared__ __align__(16) uint32_t base[];   // of each bucket: all items of smaller ones; then, behind, its items in the tiles before
     if (blockIdx.x >= tiles) return clear.block(blockIdx.x - tiles);
     wait_for_previous();
-    uint32_t *before = base + buckets;
+    const uint32_t stride = count_stride(buckets);
+    uint32_t *before = base + stride;
     const uint32_t first = blockIdx.x * kTile;
     uint2 item[kRounds];
     uint32_t rank[kRounds];
@@ -414,21 +420,29 @@ __global__ void __launch_bounds__(kTileThreads) bucket_place_kernel(Keys keys, u
         item[r] = keys.item(i);
         rank[r] = ranks[i];
     }
-    for (uint32_t b = threadIdx.x; b < buckets; b += kTileThreads) {
-        uint32_t all = 0, mine = 0;
-        if constexpr (kScanned) {
-            all = totals[b];
-            mine = counts[(uint64_t) blockIdx.x * buckets + b];
-        } else {
-#pragma unroll 16
-            for (uint32_t t = 0; t < tiles; t++) {
-                const uint32_t c = counts[t * buckets + b];
-                mine += t < blockIdx.x ? c : 0;
-                all += c;
-            }
+    if constexpr (kScanned) {
+        for (uint32_t b = threadIdx.x; b < buckets; b += kTileThreads) {
+            base[b] = totals[b];
+            before[b] = counts[(uint64_t) blockIdx.x * stride + b];
         }
-        base[b] = all;
-        before[b] = mine;
+    } else {
+        // four buckets a thread; where that leaves threads over, groups of them share the tiles
+        const uint32_t quads = stride / 4, across = min(quads, kTileThreads), groups = kTileThreads / across, group = threadIdx.x / across;
+        for (uint32_t b = threadIdx.x; b < 2 * stride; b += kTileThreads) base[b] = 0;
+        __syncthreads();
+        const uint32_t each = (tiles + groups - 1) / groups, t0 = group * each, t1 = min(t0 + each, tiles);
+        if (group < groups)
+            for (uint32_t q = threadIdx.x - group * across; q < quads; q += across) {
+                uint4 all = make_uint4(0, 0, 0, 0), mine = all;
+#pragma unroll 16
+                for (uint32_t t = t0; t < t1; t++) {
+                    const uint4 c = __ldg(reinterpret_cast<const uint4 *>(counts + t * stride) + q);
+                    all.x += c.x; all.y += c.y; all.z += c.z; all.w += c.w;
+                    if (t < blockIdx.x) { mine.x += c.x; mine.y += c.y; mine.z += c.z; mine.w += c.w; }
+                }
+                atomicAdd(base + 4 * q, all.x); atomicAdd(base + 4 * q + 1, all.y); atomicAdd(base + 4 * q + 2, all.z); atomicAdd(base + 4 * q + 3, all.w);
+                atomicAdd(before + 4 * q, mine.x); atomicAdd(before + 4 * q + 1, mine.y); atomicAdd(before + 4 * q + 2, mine.z); atomicAdd(before + 4 * q + 3, mine.w);
+            }
     }
     scan_buckets(base, buckets);
     if (blockIdx.x == 0)
@@ -977,10 +991,10 @@ cudaError_t sort_pass(const Keys &keys, uint32_t items, const Digit &digit, uint
     if (e != cudaSuccess) return e;
     c = clear();
     if (tiles <= kMaxFusedTiles)
-        return launch(bucket_place_kernel<To, false>, tiles + c.blocks(), kTileThreads, buckets * 8, stream, true, keys, items, digit, buckets, tiles, counts, totals, ranks, to, c);
+        return launch(bucket_place_kernel<To, false>, tiles + c.blocks(), kTileThreads, count_stride(buckets) * 8, stream, true, keys, items, digit, buckets, tiles, counts, totals, ranks, to, c);
     e = launch(bucket_scan_kernel, ceil_div(buckets, 32), 1024, 0, stream, true, counts, tiles, buckets, totals);
     if (e != cudaSuccess) return e;
-    return launch(bucket_place_kernel<To, true>, tiles + c.blocks(), kTileThreads, buckets * 8, stream, true, keys, items, digit, buckets, tiles, counts, totals, ranks, to, c);
+    return launch(bucket_place_kernel<To, true>, tiles + c.blocks(), kTileThreads, count_stride(buckets) * 8, stream, true, keys, items, digit, buckets, tiles, counts, totals, ranks, to, c);
 }
 
 // Scratch of the gradient: two copies of the sorted items, the counts of a pass, the partial sums of its chunks.
@@ -1007,7 +1021,7 @@ struct GradScratch {
         };
         for (int i = 0; i < 2; i++) items[i] = reinterpret_cast<uint2 *>(take(count * 8));
         ranks = reinterpret_cast<uint16_t *>(take(count * 2));
-        counts = reinterpret_cast<uint32_t *>(take((ceil_div(count, kTile) << pass_bits) * 4));
+        counts = reinterpret_cast<uint32_t *>(take(ceil_div(count, kTile) * count_stride(1u << pass_bits) * 4));
         totals = reinterpret_cast<uint32_t *>(take(4ull << pass_bits));
         partial = reinterpret_cast<float *>(take(2 * ceil_div(count, chunk) * dim * 4));
         bytes = at;
@@ -1026,7 +1040,7 @@ struct DispatchScratch {
             return static_cast<char *>(base) + here;
         };
         ranks = reinterpret_cast<uint16_t *>(take(pairs * 2));
-        counts = reinterpret_cast<uint32_t *>(take(ceil_div(pairs, kTile) * (partitions + 1) * 4));
+        counts = reinterpret_cast<uint32_t *>(take(ceil_div(pairs, kTile) * count_stride(partitions + 1) * 4));
         totals = reinterpret_cast<uint32_t *>(take((partitions + 1) * 4ull));
     }
 };
