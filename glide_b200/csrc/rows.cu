@@ -26,11 +26,10 @@ constexpr uint32_t kMaxChoices = 128;       // as many as glide_bruteforce_knn r
 constexpr uint32_t kMaxDim = 1u << 20;
 constexpr uint32_t kRounds = 8;             // items of a thread in the counting sort
 constexpr uint32_t kTileThreads = 256, kTile = kTileThreads * kRounds;
-constexpr uint32_t kOneTile = 4096;         // items that one CTA sorts in one launch
-constexpr uint32_t kMaxPassBits = 11;       // digits of a pass: the counters of kOneTile's 16 warps take 64 KB of shared memory
+constexpr uint32_t kFew = 4096;             // items that are sorted by comparing each with all
+constexpr uint32_t kMaxPassBits = 11;       // digits of a pass
 constexpr uint32_t kMaxFusedTiles = 64;     // tiles whose counts every CTA of the second kernel adds up by itself
 constexpr uint32_t kClearShare = 24u << 20; // bytes of a gradient that are cleared beside each launch of its sort
-constexpr uint32_t kSmallPairs = 2048;      // pairs that dispatch_rows places and copies in one launch
 
 // ---- rows as words ----------------------------------------------------------------------------------------
 template<int B> struct Word;
@@ -190,8 +189,8 @@ cudaError_t launch(void (*kernel)(P...), uint64_t grid, uint32_t block, uint32_t
 // A CTA takes a tile of consecutive items, each of its warps a run of 256, 32 at a time: a lane's rank among the items of
 // its digit is the warp's running count plus the equal digits at lower lanes, and a scan over the warps' counts makes it the
 // rank in the tile. No atomics: the order depends on nothing but the keys. Few launches count most here (the data are 6 to 10
-// bytes an item): kOneTile items are sorted by one launch, up to kMaxFusedTiles tiles by two launches a pass (every CTA of the
-// second adds up the counts of all tiles), more by three. Tiles are small because their items' scattered stores leave an SM at
+// bytes an item): up to kFew items are sorted by one launch that compares each with all, up to kMaxFusedTiles tiles by two launches a
+// pass (every CTA of the second adds up the counts of all tiles), more by three. Tiles are small because their items' scattered stores leave an SM at
 // one sector a cycle: with 8,192 items to a tile a pass over 100,000 ids took 31 us.
 struct Digit {
     uint32_t limit, shift, bits;   // keys beyond limit count as limit; bits: of the digit
@@ -206,29 +205,35 @@ struct Keys {
     __device__ __forceinline__ uint32_t key(uint32_t i) const { return items ? items[i].x : plain[i]; }
 };
 
-// Rows that CTAs without a tile clear while the others sort (bytes of memory that is idle then).
+// Bytes [lo, hi) from `at` on, multiples of 2, cleared by a CTA in words of 16 bytes but for the ends; `skip(first, last)` names words
+// (by their first and last byte) that are left to the caller.
+template<typename Skip>
+__device__ __forceinline__ void clear_bytes(uint8_t *at, uint64_t lo, uint64_t hi, Skip skip) {
+    const uint64_t base = reinterpret_cast<uintptr_t>(at);
+    const uint64_t up = ((base + lo + 15) & ~(uint64_t) 15) - base, down = ((base + hi) & ~(uint64_t) 15) - base;
+    const uint64_t first = up < hi ? up : hi, last = down > first && down <= hi ? down : first;
+    for (uint64_t o = first + threadIdx.x * 16ull; o < last; o += blockDim.x * 16ull)
+        if (!skip((uint32_t) (o - lo), (uint32_t) (o - lo) + 15)) __stcg(reinterpret_cast<uint4 *>(at + o), make_uint4(0, 0, 0, 0));
+    const uint32_t head = (uint32_t) (first - lo) / 2, tail = (uint32_t) (hi - last) / 2;
+    if (threadIdx.x < head + tail) {   // at most 7 halves each
+        const uint64_t o = threadIdx.x < head ? lo + 2 * threadIdx.x : last + 2 * (threadIdx.x - head);
+        if (!skip((uint32_t) (o - lo), (uint32_t) (o - lo) + 1)) *reinterpret_cast<uint16_t *>(at + o) = 0;
+    }
+}
+
+// Rows that CTAs without a tile clear while the others sort (the memory is idle then).
 struct Clear {
     uint8_t *at;
     uint64_t stride, bytes;    // of a row
     uint32_t rows, each;       // all rows, and those of a CTA
-    uint32_t word;             // 16, 4 or 2: what addresses, strides and bytes are multiples of
     __host__ __device__ uint32_t blocks() const { return rows == 0 ? 0 : (rows - 1) / each + 1; }
-    template<typename W> __device__ __forceinline__ void run(uint32_t r0, uint32_t r1) const {
-        const uint32_t words = (uint32_t) (bytes / sizeof(W));
-        W zero;
-        memset(&zero, 0, sizeof zero);
-        for (uint32_t x = threadIdx.x; x < (r1 - r0) * words; x += blockDim.x) {
-            const uint32_t r = x / words, w = x - r * words;
-            __stcg(reinterpret_cast<W *>(at + (r0 + r) * stride) + w, zero);
-        }
-    }
     // Touches nothing that the launches before it read or write, so it waits for none of them.
     __device__ __forceinline__ void block(uint32_t b) const {
         let_next_start();
-        const uint32_t r0 = b * each, r1 = min(r0 + each, rows);
-        if (word == 16) run<uint4>(r0, r1);
-        else if (word == 4) run<uint32_t>(r0, r1);
-        else run<uint16_t>(r0, r1);
+        const uint64_t r0 = b * each, r1 = min((uint32_t) r0 + each, rows);
+        const auto none = [](uint32_t, uint32_t) { return false; };
+        if (stride == bytes) return clear_bytes(at, r0 * bytes, r1 * bytes, none);
+        for (uint64_t r = r0; r < r1; r++) clear_bytes(at + r * stride, 0, bytes, none);
     }
 };
 
@@ -454,47 +459,33 @@ __global__ void __launch_bounds__(kTileThreads) bucket_place_kernel(Keys keys, u
     }
 }
 
-// One tile: ranks and places in one launch.
-template<typename To>
-__device__ __forceinline__ void sort_tile(const Keys &keys, uint32_t items, const Digit &digit, uint32_t buckets, uint32_t *base, uint16_t *warp_counts, const To &to) {
-    uint2 item[kRounds];
-    uint32_t d[kRounds], rank[kRounds];
-#pragma unroll
-    for (uint32_t r = 0; r < kRounds; r++) {
-        const uint32_t i = tile_item(r);
-        item[r] = keys.item(min(i, items - 1));
-        d[r] = i < items ? digit.of(item[r].x) : kNone;
+// Few items: an item's place is the number of smaller keys and of equal ones before it. A CTA holds all keys in shared memory, `few_keys`
+// fills them; a warp counts for one item. 4,096 items take 6 us, two passes over tiles of them 14.
+__device__ __forceinline__ void few_keys(const uint32_t *__restrict__ keys, uint32_t items, uint32_t limit, uint4 (&all)[kFew / 4]) {
+    uint32_t *to = reinterpret_cast<uint32_t *>(all);
+    for (uint32_t i = threadIdx.x; i < (items + 3) / 4 * 4; i += blockDim.x) to[i] = i < items ? min(keys[i], limit) : kNone;
+}
+__device__ __forceinline__ uint32_t few_place(const uint4 (&all)[kFew / 4], uint32_t items, uint32_t item, uint32_t key) {
+    uint32_t before = 0;
+    for (uint32_t q = threadIdx.x & 31u; q < (items + 3) / 4; q += 32) {
+        const uint4 k = all[q];
+        before += (k.x < key) + (k.y < key) + (k.z < key) + (k.w < key);
+        before += (k.x == key && 4 * q < item) + (k.y == key && 4 * q + 1 < item) + (k.z == key && 4 * q + 2 < item) + (k.w == key && 4 * q + 3 < item);
     }
-    rank_tile(d, digit.bits, buckets, warp_counts, rank, [&](uint32_t b, uint32_t sum) { base[b] = sum; });
-    scan_buckets(base, buckets);
-    for (uint32_t b = threadIdx.x; b < buckets; b += blockDim.x) to.start(b, base[b]);
-#pragma unroll
-    for (uint32_t r = 0; r < kRounds; r++)
-        if (d[r] != kNone) to.item(item[r], digit, base[d[r]] + rank[r]);
+    return __reduce_add_sync(0xffffffffu, before);
+}
+
+__global__ void __launch_bounds__(256) few_sort_kernel(const uint32_t *__restrict__ keys, uint32_t items, uint32_t limit, uint2 *__restrict__ sorted, Clear clear) {
+    __shared__ uint4 all[kFew / 4];
+    const uint32_t blocks = (items + 7) / 8;
+    if (blockIdx.x >= blocks) return clear.block(blockIdx.x - blocks);
+    wait_for_previous();
+    few_keys(keys, items, limit, all);
     __syncthreads();
-}
-
-__global__ void __launch_bounds__(kOneTile / kRounds) place_tile_kernel(Keys keys, uint32_t items, Digit digit, uint32_t buckets, ToPlaces to) {
-    extern __shared__ __align__(16) uint16_t warp_counts[];
-    uint32_t *base = reinterpret_cast<uint32_t *>(reinterpret_cast<char *>(warp_counts) + rank_smem(blockDim.x >> 5, buckets));
-    wait_for_previous();
-    sort_tile(keys, items, digit, buckets, base, warp_counts, to);
-}
-
-// All passes of a radix sort of one tile; the items lie in global memory between passes (the CTA's barriers order them).
-__global__ void __launch_bounds__(kOneTile / kRounds) sort_tile_kernel(const uint32_t *keys, uint32_t items, uint32_t limit, uint32_t bits, uint32_t pass_bits,
-                                                                       uint2 *items0, uint2 *items1, Clear clear) {
-    extern __shared__ __align__(16) uint16_t warp_counts[];
-    uint32_t *base = reinterpret_cast<uint32_t *>(reinterpret_cast<char *>(warp_counts) + rank_smem(blockDim.x >> 5, 1u << pass_bits));
-    if (blockIdx.x >= 1) return clear.block(blockIdx.x - 1);
-    wait_for_previous();
-    Keys in{keys, nullptr};
-    for (uint32_t shift = 0, pass = 0; shift < bits; shift += pass_bits, pass++) {
-        uint2 *to = pass & 1 ? items1 : items0;
-        const uint32_t here = min(pass_bits, bits - shift);
-        sort_tile(in, items, Digit{limit, shift, here}, 1u << here, base, warp_counts, ToSorted{to});
-        in = Keys{nullptr, to};
-    }
+    const uint32_t i = blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (i >= items) return;
+    const uint32_t key = reinterpret_cast<const uint32_t *>(all)[i], place = few_place(all, items, i, key);
+    if ((threadIdx.x & 31u) == 0) sorted[place] = make_uint2(key, i);
 }
 
 // ---- gradient of a lookup ---------------------------------------------------------------------------------------
@@ -505,6 +496,8 @@ struct GradArgs {
     uint64_t in_stride, out_stride;
     int accumulate;
     float *partial;                  // (2 * chunk + which) * dim: sums of runs that leave their chunk
+    uint64_t row_bytes;              // of the table's gradient, where its rows lie behind one another; otherwise 0
+    Div by_row_bytes;
     uint32_t join_blocks, clear_from, clear_rows;   // CTAs that join; the others clear clear_rows rows each, from row clear_from on
     __device__ __forceinline__ uint32_t key(uint64_t i) const { return sorted[i].x; }
 };
@@ -554,6 +547,20 @@ __device__ __forceinline__ void clear_rows(O *out, const GradArgs &a, uint32_t r
         at = a.key(at + blockDim.x - 1) == head ? first_not_below(a.sorted, at + blockDim.x, a.items, head + 1) : at + blockDim.x;
     }
     __syncthreads();
+    if (a.row_bytes >= 16) {   // a word of 16 bytes lies in two rows at most; one that lies in a named and another one goes out in halves
+        uint8_t *at_bytes = reinterpret_cast<uint8_t *>(out) + r0 * a.row_bytes;
+        const auto is_named = [&](uint32_t byte) {
+            const uint32_t r = a.by_row_bytes.of(byte);
+            return (named[r >> 5] >> (r & 31u) & 1u) != 0;
+        };
+        return clear_bytes(at_bytes, 0, (r1 - r0) * a.row_bytes, [&](uint32_t first, uint32_t last) {
+            const bool x = is_named(first), y = is_named(last);
+            if (x != y)
+                for (uint32_t o = first; o < last; o += 2)
+                    if (!is_named(o)) *reinterpret_cast<uint16_t *>(at_bytes + o) = 0;
+            return x || y;
+        });
+    }
     float zero[V];
 #pragma unroll
     for (int i = 0; i < V; i++) zero[i] = 0.0f;
@@ -721,15 +728,16 @@ __global__ void __launch_bounds__(256) dispatch_kernel(const uint8_t *__restrict
     }
 }
 
-// Few pairs: everything in one launch. A CTA owns one row; a warp finds a pair's place by comparing it with all pairs (at most
-// kSmallPairs of them, in shared memory), then the CTA copies the row. One CTA more counts the partitions.
+// Few pairs: everything in one launch. A CTA owns one row; a warp finds a pair's place by comparing it with all pairs, then the CTA
+// copies the row. One CTA more counts the partitions.
 template<int B>
 __global__ void __launch_bounds__(256) dispatch_small_kernel(const uint8_t *__restrict__ rows, uint64_t stride, uint32_t count, uint32_t words,
                                                              const uint32_t *__restrict__ choice, uint32_t choices, uint32_t partitions,
                                                              uint8_t *__restrict__ sorted, uint64_t sorted_stride, uint32_t *__restrict__ position,
                                                              uint32_t *__restrict__ map, uint32_t *__restrict__ segment_start) {
     using W = typename Word<B>::type;
-    __shared__ uint32_t keys[kSmallPairs], place[kMaxChoices];
+    __shared__ uint4 all[kFew / 4];
+    __shared__ uint32_t place[kMaxChoices];
     extern __shared__ __align__(16) uint32_t counts[];
     const uint32_t pairs = count * choices, warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, row = blockIdx.x;
     if (row == count) {
@@ -743,17 +751,14 @@ __global__ void __launch_bounds__(256) dispatch_small_kernel(const uint8_t *__re
         for (uint32_t b = threadIdx.x; b <= partitions; b += 256) segment_start[b] = counts[b];
         return;
     }
-    for (uint32_t i = threadIdx.x; i < pairs; i += 256) keys[i] = min(choice[i], partitions);
+    few_keys(choice, pairs, partitions, all);
     W w;
     memset(&w, 0, sizeof w);
     const uint8_t *from = rows + (uint64_t) row * stride;
     if (threadIdx.x < words) w = get_word<false>(reinterpret_cast<const W *>(from + (uint64_t) threadIdx.x * B));
     __syncthreads();
     for (uint32_t j = warp; j < choices; j += 8) {
-        const uint32_t pair = row * choices + j, key = keys[pair];
-        uint32_t before = 0;
-        for (uint32_t i = lane; i < pairs; i += 32) before += keys[i] < key || (keys[i] == key && i < pair);
-        before = __reduce_add_sync(0xffffffffu, before);
+        const uint32_t pair = row * choices + j, key = reinterpret_cast<const uint32_t *>(all)[pair], before = few_place(all, pairs, pair, key);
         if (lane == 0) {
             const bool there = key < partitions;
             place[j] = position[pair] = there ? before : kNone;
@@ -807,8 +812,10 @@ __global__ void __launch_bounds__(256) combine_kernel(const T *__restrict__ sort
     store<T, V>(out + (uint64_t) row * out_stride + at, acc);
 }
 
-// grad_sorted[position[t,j]] = weight[t,j] * grad[t] and grad_weights[t,j] = <grad[t], sorted[position[t,j]]>: G lanes own a row.
-template<typename T, int V, int K, int G>
+// grad_sorted[position[t,j]] = weight[t,j] * grad[t] and grad_weights[t,j] = <grad[t], sorted[position[t,j]]>: G lanes own a row,
+// and have U of its words and those of K of its places in flight. A warp a row beats a CTA a row (16,384 x 8 rows of 4 KB: 180 against
+// 205 us; 39,047 x 4 of 5 KB: 278 against 340) but where rows are few (64 x 8: 9.1 against 3.3; 1,000 x 4 of 8 KB: 22 against 16).
+template<typename T, int V, int K, int U, int G>
 __global__ void __launch_bounds__(256) combine_grad_kernel(const T *__restrict__ grad, uint64_t grad_stride, uint32_t count, uint32_t words,
                                                            const T *__restrict__ sorted, uint64_t stride, uint32_t sorted_rows,
                                                            const uint32_t *__restrict__ position, uint32_t choices,
@@ -827,23 +834,34 @@ __global__ void __launch_bounds__(256) combine_grad_kernel(const T *__restrict__
             w[j] = weights && j0 + j < choices ? weights[pair] : 1.0f;
             dot[j] = 0.0f;
         }
-        for (uint32_t c = l; c < words; c += G) {
-            float g[V];
-            WordOf<T, V> y[K];
+        for (uint32_t c0 = l; c0 < words; c0 += G * U) {
+            WordOf<T, V> x[U], y[U][K];
 #pragma unroll
-            for (int j = 0; j < K; j++) y[j] = get_word_if<WordOf<T, V>>(sorted + (uint64_t) p[j] * stride + (uint64_t) c * V, p[j] < sorted_rows);
-            load<T, V>(grad + (uint64_t) row * grad_stride + (uint64_t) c * V, g);
+            for (int u = 0; u < U; u++) {
+                const uint32_t c = c0 + u * G;
+                const bool in = u == 0 || c < words;
+                x[u] = get_word_if<WordOf<T, V>>(grad + (uint64_t) row * grad_stride + (uint64_t) c * V, in);
 #pragma unroll
-            for (int j = 0; j < K; j++) {
-                if (p[j] >= sorted_rows) continue;
-                float f[V], o[V];
-                unpack<T, V>(y[j], f);
+                for (int j = 0; j < K; j++) y[u][j] = get_word_if<WordOf<T, V>>(sorted + (uint64_t) p[j] * stride + (uint64_t) c * V, in && p[j] < sorted_rows);
+            }
 #pragma unroll
-                for (int i = 0; i < V; i++) {
-                    dot[j] = fmaf(g[i], f[i], dot[j]);
-                    o[i] = w[j] * g[i];
+            for (int u = 0; u < U; u++) {
+                const uint32_t c = c0 + u * G;
+                if (u > 0 && c >= words) break;
+                float g[V];
+                unpack<T, V>(x[u], g);
+#pragma unroll
+                for (int j = 0; j < K; j++) {
+                    if (p[j] >= sorted_rows) continue;
+                    float f[V], o[V];
+                    unpack<T, V>(y[u][j], f);
+#pragma unroll
+                    for (int i = 0; i < V; i++) {
+                        dot[j] = fmaf(g[i], f[i], dot[j]);
+                        o[i] = w[j] * g[i];
+                    }
+                    store<T, V>(grad_sorted + (uint64_t) p[j] * grad_sorted_stride + (uint64_t) c * V, o);
                 }
-                store<T, V>(grad_sorted + (uint64_t) p[j] * grad_sorted_stride + (uint64_t) c * V, o);
             }
         }
 #pragma unroll
@@ -1033,7 +1051,7 @@ struct DispatchScratch {
     uint16_t *ranks = nullptr;
     uint64_t bytes = 0;
     DispatchScratch(void *base, uint64_t pairs, uint32_t partitions) {
-        if (pairs <= kOneTile) return;
+        if (pairs <= kFew) return;
         auto take = [&](uint64_t size) {
             const uint64_t here = bytes;
             bytes += align256(size);
@@ -1109,20 +1127,16 @@ int glide_lookup_rows_grad(glide_ctx *ctx, const void *d_grad, int row_type, uin
     clear_each = clear_each < 1 ? 1 : clear_each > 256 ? 256 : clear_each;
     const uint64_t share = accumulate || count >= n / 2 ? 0 : kClearShare / row_bytes;
     auto clear = [&]() {
-        Clear c{static_cast<uint8_t *>(d_table_grad) + (uint64_t) cleared * table_grad_stride * bytes_of(grad_type), table_grad_stride * bytes_of(grad_type), row_bytes,
-                (uint32_t) (share < n - cleared ? share : n - cleared), clear_each, 2};
-        const uint64_t any = reinterpret_cast<uintptr_t>(c.at) | c.stride | c.bytes;
-        c.word = any % 16 == 0 ? 16 : any % 4 == 0 ? 4 : 2;
+        const Clear c{static_cast<uint8_t *>(d_table_grad) + (uint64_t) cleared * table_grad_stride * bytes_of(grad_type), table_grad_stride * bytes_of(grad_type), row_bytes,
+                      (uint32_t) (share < n - cleared ? share : n - cleared), clear_each};
         cleared += c.rows;
         return c;
     };
     const uint2 *sorted = nullptr;
-    if (count > 0 && count <= kOneTile) {
-        const uint32_t threads = (uint32_t) ceil_div(items, kRounds * 32) * 32;
+    if (count > 0 && count <= kFew) {
         const Clear c = clear();
-        ROWS_CUDA(launch(sort_tile_kernel, 1 + c.blocks(), threads, rank_smem(threads / 32, 1u << w.pass_bits) + (4u << w.pass_bits), s, false, d_ids, items, (uint32_t) n, w.bits, w.pass_bits,
-                         w.items[0], w.items[1], c));
-        sorted = w.items[(w.passes - 1) & 1];
+        ROWS_CUDA(launch(few_sort_kernel, ceil_div(items, 8) + c.blocks(), 256, 0, s, false, d_ids, items, (uint32_t) n, w.items[0], c));
+        sorted = w.items[0];
     } else if (count > 0) {
         for (uint32_t pass = 0; pass < w.passes; pass++) {
             const uint32_t left = w.bits - pass * w.pass_bits, here = left < w.pass_bits ? left : w.pass_bits;
@@ -1131,7 +1145,7 @@ int glide_lookup_rows_grad(glide_ctx *ctx, const void *d_grad, int row_type, uin
         }
     }
     const uint32_t most = most_of(row_type), v0 = count ? in.width(most) : most, v1 = out.width(most), v = v0 < v1 ? v0 : v1;
-    GradArgs a{sorted, items, (uint32_t) n, dim, dim / v, 32, 1, w.chunk, scale, grad_stride, table_grad_stride, accumulate, w.partial, 0, cleared, clear_each};
+    GradArgs a{sorted, items, (uint32_t) n, dim, dim / v, 32, 1, w.chunk, scale, grad_stride, table_grad_stride, accumulate, w.partial, table_grad_stride == dim ? row_bytes : 0, Div(row_bytes), 0, cleared, clear_each};
     while (a.lanes > 1 && a.lanes / 2 >= a.words) a.lanes /= 2;
     a.slabs = (uint32_t) ceil_div(a.words, a.lanes);
     const uint64_t chunks = ceil_div(items, a.chunk), join = ceil_div(chunks * a.slabs * a.lanes, 256), units = chunks < 2 ? 0 : (chunks - 1) * a.slabs;
@@ -1196,7 +1210,7 @@ int glide_dispatch_rows(glide_ctx *ctx, const void *d_rows, int row_type, uint64
             default: return run(Width<2>{});
         }
     };
-    if (pairs <= kSmallPairs) {
+    if (pairs <= kFew) {
         ROWS_CUDA(with_bytes([&](auto b) {
             return launch(dispatch_small_kernel<decltype(b)::value>, count + 1, 256, (partitions + 1) * 4, s, false, from, row_stride * e, (uint32_t) count, words, d_choice, choices, partitions,
                           to, sorted_stride * e, d_position, d_map, d_segment_start);
@@ -1206,12 +1220,7 @@ int glide_dispatch_rows(glide_ctx *ctx, const void *d_rows, int row_type, uint64
     const DispatchScratch w(d_workspace, pairs, partitions);
     const Digit digit{partitions, 0, bits_for(partitions + 1)};
     const ToPlaces places{d_position, d_map, d_segment_start, Div(choices)};
-    if (pairs <= kOneTile) {
-        const uint32_t threads = (uint32_t) ceil_div(pairs, kRounds * 32) * 32;
-        ROWS_CUDA(launch(place_tile_kernel, 1, threads, rank_smem(threads / 32, partitions + 1) + (partitions + 1) * 4, s, false, Keys{d_choice, nullptr}, (uint32_t) pairs, digit, partitions + 1, places));
-    } else {
-        ROWS_CUDA(sort_pass(Keys{d_choice, nullptr}, (uint32_t) pairs, digit, partitions + 1, w.counts, w.totals, w.ranks, places, false, s, [] { return Clear{}; }));
-    }
+    ROWS_CUDA(sort_pass(Keys{d_choice, nullptr}, (uint32_t) pairs, digit, partitions + 1, w.counts, w.totals, w.ranks, places, false, s, [] { return Clear{}; }));
     const uint64_t each = 0x7fff0000u / words;   // rows of a launch: its words are counted in 31 bits
     for (uint64_t r0 = 0; r0 < count; r0 += each) {
         const uint32_t rows = (uint32_t) (count - r0 < each ? count - r0 : each), units = rows * words;
@@ -1290,15 +1299,14 @@ int glide_combine_rows_grad(glide_ctx *ctx, const void *d_grad, int row_type, ui
     ROWS_CUDA(with_rows(row_type, v, [&](auto t, auto wd) {
         using T = decltype(t);
         constexpr int V = decltype(wd)::value;
-        auto go = [&](auto kk, auto gg) {
-            constexpr int K = decltype(kk)::value, G = decltype(gg)::value;
-            combine_grad_kernel<T, V, K, G><<<(uint32_t) ceil_div(count, 256 / G), 256, 0, s>>>(
-                static_cast<const T *>(d_grad), grad_stride, (uint32_t) count, words, static_cast<const T *>(d_sorted), sorted_stride, (uint32_t) sorted_rows, d_position, choices,
-                d_weights_or_null, static_cast<T *>(d_grad_sorted), grad_sorted_stride, d_grad_weights_or_null);
-            return cudaGetLastError();
+        auto go = [&](auto kk, auto uu, auto gg) {
+            constexpr int K = decltype(kk)::value, U = decltype(uu)::value, G = decltype(gg)::value;
+            return launch(combine_grad_kernel<T, V, K, U, G>, ceil_div(count, 256 / G), 256, 0, s, false, static_cast<const T *>(d_grad), grad_stride, (uint32_t) count, words,
+                          static_cast<const T *>(d_sorted), sorted_stride, (uint32_t) sorted_rows, d_position, choices, d_weights_or_null, static_cast<T *>(d_grad_sorted),
+                          grad_sorted_stride, d_grad_weights_or_null);
         };
-        if (choices <= 2) return words > 64 ? go(Width<2>{}, Width<256>{}) : go(Width<2>{}, Width<32>{});
-        return words > 64 ? go(Width<8>{}, Width<256>{}) : go(Width<8>{}, Width<32>{});
+        if (count <= 148 * 8 && words > 64) return choices <= 4 ? go(Width<4>{}, Width<1>{}, Width<256>{}) : go(Width<8>{}, Width<1>{}, Width<256>{});
+        return choices <= 2 ? go(Width<2>{}, Width<2>{}, Width<32>{}) : choices < 8 ? go(Width<4>{}, Width<1>{}, Width<32>{}) : go(Width<8>{}, Width<1>{}, Width<32>{});
     }));
     return GLIDE_OK;
 }
