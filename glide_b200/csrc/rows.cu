@@ -27,6 +27,8 @@ constexpr uint32_t kMaxDim = 1u << 20;
 constexpr uint32_t kRounds = 8;             // items of a thread in the counting sort
 constexpr uint32_t kTileThreads = 256, kTile = kTileThreads * kRounds;
 constexpr uint32_t kFew = 4096;             // items that are sorted by comparing each with all
+constexpr uint32_t kFewPairs = 2048;        // pairs that dispatch_rows places and copies in one launch (2,000: 6 to 8 us, by tiles 8)
+constexpr uint32_t kFewIds = 1024;          // ids whose gradient takes one launch
 constexpr uint32_t kMaxPassBits = 11;       // digits of a pass
 constexpr uint32_t kMaxFusedTiles = 64;     // tiles whose counts every CTA of the second kernel adds up by itself
 constexpr uint32_t kClearShare = 24u << 20; // bytes of a gradient that are cleared beside each launch of its sort
@@ -461,16 +463,30 @@ __global__ void __launch_bounds__(kTileThreads) bucket_place_kernel(Keys keys, u
 
 // Few items: an item's place is the number of smaller keys and of equal ones before it. A CTA holds all keys in shared memory, `few_keys`
 // fills them; a warp counts for one item. 4,096 items take 6 us, two passes over tiles of them 14.
-__device__ __forceinline__ void few_keys(const uint32_t *__restrict__ keys, uint32_t items, uint32_t limit, uint4 (&all)[kFew / 4]) {
+__device__ __forceinline__ void few_keys(const uint32_t *__restrict__ keys, uint32_t items, uint32_t limit, uint4 *all) {
     uint32_t *to = reinterpret_cast<uint32_t *>(all);
+#pragma unroll 8
     for (uint32_t i = threadIdx.x; i < (items + 3) / 4 * 4; i += blockDim.x) to[i] = i < items ? min(keys[i], limit) : kNone;
 }
-__device__ __forceinline__ uint32_t few_place(const uint4 (&all)[kFew / 4], uint32_t items, uint32_t item, uint32_t key) {
-    uint32_t before = 0;
-    for (uint32_t q = threadIdx.x & 31u; q < (items + 3) / 4; q += 32) {
+__device__ __forceinline__ uint32_t few_place(const uint4 *all, uint32_t items, uint32_t item, uint32_t key) {
+    // keys before the item count when they are not greater, those behind it when they are smaller
+    const uint32_t lane = threadIdx.x & 31u, quads = (items + 3) / 4, own = item / 4;
+    uint32_t before = 0, q = lane;
+#pragma unroll 4
+    for (; q < own; q += 32) {
+        const uint4 k = all[q];
+        before += (k.x <= key) + (k.y <= key) + (k.z <= key) + (k.w <= key);
+    }
+    if (q == own) {
+        const uint4 k = all[q];
+        const uint32_t in = item & 3u;
+        before += (in > 0 ? k.x <= key : 0) + (in > 1 ? k.y <= key : k.y < key) + (in > 2 ? k.z <= key : k.z < key) + (k.w < key);
+        q += 32;
+    }
+#pragma unroll 4
+    for (; q < quads; q += 32) {
         const uint4 k = all[q];
         before += (k.x < key) + (k.y < key) + (k.z < key) + (k.w < key);
-        before += (k.x == key && 4 * q < item) + (k.y == key && 4 * q + 1 < item) + (k.z == key && 4 * q + 2 < item) + (k.w == key && 4 * q + 3 < item);
     }
     return __reduce_add_sync(0xffffffffu, before);
 }
@@ -530,22 +546,35 @@ __device__ __forceinline__ uint32_t first_not_below(const uint2 *__restrict__ so
     return lo;
 }
 
-// Rows [r0, r1) that no id names are cleared.
-template<typename O, int V>
-__device__ __forceinline__ void clear_rows(O *out, const GradArgs &a, uint32_t r0, uint32_t r1) {
-    __shared__ uint32_t named[256 / 32];   // a CTA clears 256 rows at most
-    if (threadIdx.x < 8) named[threadIdx.x] = 0;
-    __syncthreads();
+// Of rows [r0, r1), at most 256, those that an id names: by the sorted items.
+__device__ __forceinline__ void name_rows(const GradArgs &a, uint32_t r0, uint32_t r1, uint32_t *named) {
     uint32_t at = first_not_below(a.sorted, 0, a.items, r0);
-    while (at < a.items) {
+    bool more = at < a.items;
+    for (int step = 0; step < 2 && more; step++) {   // mostly a few items: all of them are looked at
         const uint32_t i = at + threadIdx.x, key = i < a.items ? a.key(i) : kNone;
         if (key < r1) atomicOr(&named[(key - r0) >> 5], 1u << ((key - r0) & 31u));
-        const uint32_t here = __syncthreads_count(key < r1);
-        if (here < blockDim.x) break;
-        // a whole CTA's width of one id: on to the next id
-        const uint32_t head = a.key(at);
-        at = a.key(at + blockDim.x - 1) == head ? first_not_below(a.sorted, at + blockDim.x, a.items, head + 1) : at + blockDim.x;
+        more = __syncthreads_count(key < r1) == blockDim.x;
+        at += blockDim.x;
     }
+    if (more && r0 + threadIdx.x < r1) {   // ids that come often: each row is searched for
+        const uint32_t r = r0 + threadIdx.x;
+        uint32_t lo = at, hi = a.items;
+        while (lo < hi) {
+            const uint32_t mid = lo + (hi - lo) / 2;
+            if (a.key(mid) < r) lo = mid + 1;
+            else hi = mid;
+        }
+        if (lo < a.items && a.key(lo) == r) atomicOr(&named[(r - r0) >> 5], 1u << ((r - r0) & 31u));
+    }
+}
+
+// Rows [r0, r1) that `mark` does not name are cleared.
+template<typename O, int V, typename Mark>
+__device__ __forceinline__ void clear_rows(O *out, const GradArgs &a, uint32_t r0, uint32_t r1, Mark mark) {
+    __shared__ uint32_t named[256 / 32];
+    if (threadIdx.x < 8) named[threadIdx.x] = 0;
+    __syncthreads();
+    mark(named);
     __syncthreads();
     if (a.row_bytes >= 16) {   // a word of 16 bytes lies in two rows at most; one that lies in a named and another one goes out in halves
         uint8_t *at_bytes = reinterpret_cast<uint8_t *>(out) + r0 * a.row_bytes;
@@ -573,13 +602,13 @@ __device__ __forceinline__ void clear_rows(O *out, const GradArgs &a, uint32_t r
 // A group of lanes joins a chunk of sorted items over a slab of the row: the sum of a run of equal ids goes to the id's row, or,
 // where the run goes on in another chunk, to the chunk's partial sums (first: it came from the chunk before).
 template<typename T, typename O, int V>
-__global__ void __launch_bounds__(256) grad_join_kernel(const T *__restrict__ grad, O *__restrict__ out, GradArgs a) {
-    constexpr int U = 8;
+__global__ void __launch_bounds__(256, 4) grad_join_kernel(const T *__restrict__ grad, O *__restrict__ out, GradArgs a) {
+    constexpr int U = 4;
     wait_for_previous();
     if (blockIdx.x >= a.join_blocks) {
         const uint64_t r0 = a.clear_from + (uint64_t) (blockIdx.x - a.join_blocks) * a.clear_rows;
-        clear_rows<O, V>(out, a, (uint32_t) r0, (uint32_t) min((uint64_t) a.n, r0 + a.clear_rows));
-        return;
+        const uint32_t r1 = (uint32_t) min((uint64_t) a.n, r0 + a.clear_rows);
+        return clear_rows<O, V>(out, a, (uint32_t) r0, r1, [&](uint32_t *named) { name_rows(a, (uint32_t) r0, r1, named); });
     }
     const uint32_t group = (blockIdx.x * 256 + threadIdx.x) / a.lanes, lane = threadIdx.x & (a.lanes - 1);
     const uint32_t chunk = group / a.slabs, word = (group - chunk * a.slabs) * a.lanes + lane;
@@ -596,17 +625,19 @@ __global__ void __launch_bounds__(256) grad_join_kernel(const T *__restrict__ gr
         if (from_left || to_right) store<float, V>(a.partial + (2ull * chunk + (from_left ? 0 : 1)) * a.dim + at, acc);
         else put_grad<O, V>(out, a, id, at, acc);
     };
+    uint2 next[U];   // items of the batch to come: their rows can be fetched without waiting for them
+#pragma unroll
+    for (int u = 0; u < U; u++) next[u] = __ldg(a.sorted + min((uint32_t) c0 + u, c1 - 1));
     for (uint32_t c = (uint32_t) c0; c < c1; c += U) {
-        uint32_t key[U], value[U];
+        uint32_t key[U];
         WordOf<T, V> w[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const uint2 item = __ldg(a.sorted + min(c + u, c1 - 1));
-            key[u] = item.x;
-            value[u] = item.y;
+            key[u] = next[u].x;
+            w[u] = get_word_if<WordOf<T, V>>(grad + (uint64_t) next[u].y * a.in_stride + at, key[u] < a.n && c + u < c1);
         }
 #pragma unroll
-        for (int u = 0; u < U; u++) w[u] = get_word_if<WordOf<T, V>>(grad + (uint64_t) value[u] * a.in_stride + at, key[u] < a.n);
+        for (int u = 0; u < U; u++) next[u] = __ldg(a.sorted + min(c + U + u, c1 - 1));
 #pragma unroll
         for (int u = 0; u < U; u++) {
             if (c + u >= c1) break;
@@ -628,9 +659,89 @@ __global__ void __launch_bounds__(256) grad_join_kernel(const T *__restrict__ gr
     put(c1 < a.items && a.key(c1) == id);
 }
 
+// Few ids: everything in one launch. A CTA owns one id, unless an earlier one is equal: it lists the equal ones in order, its groups of
+// lanes add consecutive parts of the list and the groups' sums are added in order. The other CTAs clear the rows that no id names.
+// 1,000 ids: see the table of kFewIds below. An id that is most of them is one CTA's work: at worst, 1,024 equal ids of 8 KB rows, 60 us.
+template<typename T, typename O, int V>
+__global__ void __launch_bounds__(256) grad_few_kernel(const T *__restrict__ grad, O *__restrict__ out, const uint32_t *__restrict__ ids, GradArgs a) {
+    constexpr int U = 8;
+    __shared__ uint32_t keys[kFewIds], counts[8];
+    __shared__ uint16_t list[kFewIds];
+    __shared__ float part[256][V];
+    for (uint32_t i = threadIdx.x; i < a.items; i += 256) keys[i] = ids[i];
+    __syncthreads();
+    if (blockIdx.x >= a.items) {
+        const uint64_t r0 = (uint64_t) (blockIdx.x - a.items) * a.clear_rows;
+        const uint32_t r1 = (uint32_t) min((uint64_t) a.n, r0 + a.clear_rows);
+        return clear_rows<O, V>(out, a, (uint32_t) r0, r1, [&](uint32_t *named) {
+            for (uint32_t i = threadIdx.x; i < a.items; i += 256)
+                if (keys[i] >= r0 && keys[i] < r1) atomicOr(&named[(keys[i] - (uint32_t) r0) >> 5], 1u << ((keys[i] - (uint32_t) r0) & 31u));
+        });
+    }
+    const uint32_t id = keys[blockIdx.x], warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    bool earlier = id >= a.n;
+    for (uint32_t i = threadIdx.x; i < blockIdx.x; i += 256) earlier |= keys[i] == id;
+    if (__syncthreads_or(earlier)) return;
+    const uint32_t segment = (a.items + 7) / 8, i0 = min(warp * segment, a.items), i1 = min(i0 + segment, a.items);
+    uint32_t found = 0;
+    for (uint32_t i = i0; i < i1; i += 32) found += __popc(__ballot_sync(0xffffffffu, i + lane < i1 && keys[i + lane] == id));
+    if (lane == 0) counts[warp] = found;
+    __syncthreads();
+    uint32_t all = 0, at = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < 8; w++) {
+        at += w < warp ? counts[w] : 0;
+        all += counts[w];
+    }
+    for (uint32_t i = i0; i < i1; i += 32) {
+        const bool equal = i + lane < i1 && keys[i + lane] == id;
+        const uint32_t lanes = __ballot_sync(0xffffffffu, equal);
+        if (equal) list[at + __popc(lanes & ((1u << lane) - 1))] = (uint16_t) (i + lane);
+        at += __popc(lanes);
+    }
+    __syncthreads();
+    const uint32_t group = threadIdx.x / a.lanes, groups = 256 / a.lanes, each = (all + groups - 1) / groups;
+    const uint32_t s0 = min(group * each, all), s1 = min(s0 + each, all);
+    for (uint32_t word = threadIdx.x & (a.lanes - 1); word < a.words; word += a.lanes) {   // more than once only where one group has the row
+        float acc[V];
+#pragma unroll
+        for (int i = 0; i < V; i++) acc[i] = 0.0f;
+        for (uint32_t s = s0; s < s1; s += U) {
+            WordOf<T, V> w[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) w[u] = get_word_if<WordOf<T, V>>(grad + (uint64_t) list[min(s + u, s1 - 1)] * a.in_stride + word * V, s + u < s1);
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                if (s + u >= s1) break;
+                float f[V];
+                unpack<T, V>(w[u], f);
+#pragma unroll
+                for (int i = 0; i < V; i++) acc[i] += f[i];
+            }
+        }
+        if (groups == 1) {
+            put_grad<O, V>(out, a, id, word * V, acc);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; i++) part[threadIdx.x][i] = acc[i];
+        }
+    }
+    if (groups == 1) return;
+    __syncthreads();
+    if (threadIdx.x >= a.words) return;   // fewer than a group's lanes: the first group
+    float acc[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) acc[i] = part[threadIdx.x][i];
+    const uint32_t used = (all + each - 1) / each;
+    for (uint32_t g = 1; g < used; g++)
+#pragma unroll
+        for (int i = 0; i < V; i++) acc[i] += part[g * a.lanes + threadIdx.x][i];
+    put_grad<O, V>(out, a, id, threadIdx.x * V, acc);
+}
+
 // Runs over several chunks, whose first chunk's unit (a chunk and a slab) adds their partial sums and writes the row. A warp owns a unit and
-// adds short runs by itself, in order; of a run with more partial sums than kLongRun each of the CTA's eight warps takes an
-// eighth, in order, and their sums are added in order. The shape of a sum depends on the run alone.
+// adds short runs by itself, in order; the CTA's warps share the runs with more partial sums than kLongRun, each takes consecutive ones,
+// and the warps' sums are added in order.
 constexpr uint32_t kLongRun = 32;
 template<typename O, int V>
 __global__ void __launch_bounds__(256) grad_fix_kernel(O *__restrict__ out, GradArgs a, uint32_t units) {
@@ -677,11 +788,18 @@ __global__ void __launch_bounds__(256) grad_fix_kernel(O *__restrict__ out, Grad
     }
     if (lane == 0) long_last[warp] = last;
     if (!__syncthreads_or(last)) return;
-    for (uint32_t u = 0; u < 8; u++) {
-        if (long_last[u] == 0) continue;
+    // the CTA's long runs, one after another or, two or four, at once: `each` warps to a run
+    uint32_t found = 0, units_of[8];
+#pragma unroll
+    for (uint32_t u = 0; u < 8; u++)
+        if (long_last[u] != 0) units_of[found++] = u;
+    const uint32_t at_once = found >= 4 ? 4 : found >= 2 ? 2 : 1, each = 8 / at_once, share = warp & (each - 1);
+    for (uint32_t f = 0; f < found; f += at_once) {
+        const bool there = f + warp / each < found;
+        const uint32_t u = units_of[there ? f + warp / each : 0];
         const uint32_t chunk = (blockIdx.x * 8 + u) / a.slabs, word = (blockIdx.x * 8 + u - chunk * a.slabs) * a.lanes + lane;
-        const uint32_t sums = long_last[u] - chunk + 1, each = (sums + 7) / 8, s0 = min(warp * each, sums), s1 = min(s0 + each, sums);
-        const bool mine = lane < a.lanes && word < a.words;
+        const uint32_t sums = long_last[u] - chunk + 1, part_sums = (sums + each - 1) / each, s0 = min(share * part_sums, sums), s1 = min(s0 + part_sums, sums);
+        const bool mine = there && lane < a.lanes && word < a.words;
         float acc[V];
         if (mine) {
             add(chunk, word * V, s0, s1, acc);
@@ -689,11 +807,10 @@ __global__ void __launch_bounds__(256) grad_fix_kernel(O *__restrict__ out, Grad
             for (int i = 0; i < V; i++) part[warp][lane][i] = acc[i];
         }
         __syncthreads();
-        if (warp == 0 && mine) {
+        if (share == 0 && mine) {
+            for (uint32_t w = 1; w < each; w++)
 #pragma unroll
-            for (int w = 1; w < 8; w++)
-#pragma unroll
-                for (int i = 0; i < V; i++) acc[i] += part[w][lane][i];
+                for (int i = 0; i < V; i++) acc[i] += part[warp + w][lane][i];
             put_grad<O, V>(out, a, a.key((uint64_t) (chunk + 1) * a.chunk - 1), word * V, acc);
         }
         __syncthreads();
@@ -736,7 +853,7 @@ __global__ void __launch_bounds__(256) dispatch_small_kernel(const uint8_t *__re
                                                              uint8_t *__restrict__ sorted, uint64_t sorted_stride, uint32_t *__restrict__ position,
                                                              uint32_t *__restrict__ map, uint32_t *__restrict__ segment_start) {
     using W = typename Word<B>::type;
-    __shared__ uint4 all[kFew / 4];
+    __shared__ uint4 all[kFewPairs / 4];
     __shared__ uint32_t place[kMaxChoices];
     extern __shared__ __align__(16) uint32_t counts[];
     const uint32_t pairs = count * choices, warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, row = blockIdx.x;
@@ -1028,9 +1145,9 @@ struct GradScratch {
         passes = (bits + kMaxPassBits - 1) / kMaxPassBits;
         pass_bits = (bits + passes - 1) / passes;
         // Long chunks leave few partial sums, short ones many groups of lanes to work: as long as some 32 warps an SM remain
-        // (counted for words of 16 bytes of bf16).
-        chunk = 32;
-        while (chunk < 128 && count * ceil_div(dim, 256) / chunk >= 2 * 148 * 32) chunk *= 2;
+        // (counted for words of 16 bytes of bf16), 8 to 128.
+        chunk = 8;
+        while (chunk < 128 && count * dim / 256 / chunk >= 2 * 148 * 32) chunk *= 2;
         uint64_t at = 0;
         auto take = [&](uint64_t size) {
             const uint64_t here = at;
@@ -1051,7 +1168,7 @@ struct DispatchScratch {
     uint16_t *ranks = nullptr;
     uint64_t bytes = 0;
     DispatchScratch(void *base, uint64_t pairs, uint32_t partitions) {
-        if (pairs <= kFew) return;
+        if (pairs <= kFewPairs) return;
         auto take = [&](uint64_t size) {
             const uint64_t here = bytes;
             bytes += align256(size);
@@ -1096,7 +1213,7 @@ int glide_lookup_rows(glide_ctx *ctx, const void *d_table, int row_type, uint64_
 
 size_t glide_lookup_rows_grad_workspace(uint64_t n, uint32_t dim, uint64_t count) {
     if (n > kNone || dim > kMaxDim || count > 0x7fffffffu) return 0;
-    return count == 0 ? 0 : (size_t) GradScratch(nullptr, n, count, dim).bytes;
+    return count <= kFewIds ? 0 : (size_t) GradScratch(nullptr, n, count, dim).bytes;
 }
 
 int glide_lookup_rows_grad(glide_ctx *ctx, const void *d_grad, int row_type, uint64_t grad_stride, const uint32_t *d_ids, uint64_t count,
@@ -1119,12 +1236,28 @@ int glide_lookup_rows_grad(glide_ctx *ctx, const void *d_grad, int row_type, uin
     const OnDevice guard(ctx->device);
     ROWS_CUDA(guard.status);
     auto s = static_cast<cudaStream_t>(stream);
+    const uint32_t most = most_of(row_type), v0 = count ? in.width(most) : most, v1 = out.width(most), v = v0 < v1 ? v0 : v1;
     const GradScratch w(d_workspace, n, count, dim);
     const uint32_t items = (uint32_t) count, row_bytes = dim * bytes_of(grad_type);
     // Rows are cleared where the memory is idle: a share with each launch of the sort, whether an id names them or not, as long as ids are
     // few beside rows; the rest by the kernel that joins, which by then knows the rows that no id names.
     uint32_t clear_each = (128u << 10) / row_bytes, cleared = 0;   // a CTA clears up to 128 KB
     clear_each = clear_each < 1 ? 1 : clear_each > 256 ? 256 : clear_each;
+    GradArgs a{nullptr, items, (uint32_t) n, dim, dim / v, 32, 1, w.chunk, scale, grad_stride, table_grad_stride, accumulate, w.partial, table_grad_stride == dim ? row_bytes : 0, Div(row_bytes), 0, 0, clear_each};
+    if (count <= kFewIds) {
+        a.lanes = 256;
+        while (a.lanes > 1 && a.lanes / 2 >= a.words) a.lanes /= 2;
+        const uint64_t grid = count + (accumulate ? 0 : ceil_div(n, clear_each));
+        if (grid == 0) return GLIDE_OK;
+        auto run = [&](auto t, auto o, auto wd) {
+            using T = decltype(t);
+            using O = decltype(o);
+            constexpr int V = decltype(wd)::value;
+            return launch(grad_few_kernel<T, O, V>, grid, 256, 0, s, false, static_cast<const T *>(d_grad), static_cast<O *>(d_table_grad), d_ids, a);
+        };
+        ROWS_CUDA(with_rows(row_type, v, [&](auto t, auto wd) { return grad_type == GLIDE_ROW_F32 ? run(t, float{}, wd) : run(t, t, wd); }));
+        return GLIDE_OK;
+    }
     const uint64_t share = accumulate || count >= n / 2 ? 0 : kClearShare / row_bytes;
     auto clear = [&]() {
         const Clear c{static_cast<uint8_t *>(d_table_grad) + (uint64_t) cleared * table_grad_stride * bytes_of(grad_type), table_grad_stride * bytes_of(grad_type), row_bytes,
@@ -1133,31 +1266,30 @@ int glide_lookup_rows_grad(glide_ctx *ctx, const void *d_grad, int row_type, uin
         return c;
     };
     const uint2 *sorted = nullptr;
-    if (count > 0 && count <= kFew) {
+    if (count <= kFew) {
         const Clear c = clear();
         ROWS_CUDA(launch(few_sort_kernel, ceil_div(items, 8) + c.blocks(), 256, 0, s, false, d_ids, items, (uint32_t) n, w.items[0], c));
         sorted = w.items[0];
-    } else if (count > 0) {
+    } else {
         for (uint32_t pass = 0; pass < w.passes; pass++) {
             const uint32_t left = w.bits - pass * w.pass_bits, here = left < w.pass_bits ? left : w.pass_bits;
             ROWS_CUDA(sort_pass(Keys{d_ids, sorted}, items, Digit{(uint32_t) n, pass * w.pass_bits, here}, 1u << here, w.counts, w.totals, w.ranks, ToSorted{w.items[pass & 1]}, pass > 0, s, clear));
             sorted = w.items[pass & 1];
         }
     }
-    const uint32_t most = most_of(row_type), v0 = count ? in.width(most) : most, v1 = out.width(most), v = v0 < v1 ? v0 : v1;
-    GradArgs a{sorted, items, (uint32_t) n, dim, dim / v, 32, 1, w.chunk, scale, grad_stride, table_grad_stride, accumulate, w.partial, table_grad_stride == dim ? row_bytes : 0, Div(row_bytes), 0, cleared, clear_each};
+    a.sorted = sorted;
+    a.clear_from = cleared;
     while (a.lanes > 1 && a.lanes / 2 >= a.words) a.lanes /= 2;
     a.slabs = (uint32_t) ceil_div(a.words, a.lanes);
     const uint64_t chunks = ceil_div(items, a.chunk), join = ceil_div(chunks * a.slabs * a.lanes, 256), units = chunks < 2 ? 0 : (chunks - 1) * a.slabs;
     const uint64_t zero = accumulate ? 0 : ceil_div(n - cleared, clear_each);
     ROWS_REQUIRE(join <= 0xffffffu && units <= 0x7fffffffu && join + zero <= 0x7fffffffu, GLIDE_ERR_UNSUPPORTED, "lookup_rows_grad: too many values in one call");   // threads are counted in 32 bits
     a.join_blocks = (uint32_t) join;
-    if (join + zero == 0) return GLIDE_OK;
     auto run = [&](auto t, auto o, auto wd) {
         using T = decltype(t);
         using O = decltype(o);
         constexpr int V = decltype(wd)::value;
-        const cudaError_t e = launch(grad_join_kernel<T, O, V>, join + zero, 256, 0, s, count > 0, static_cast<const T *>(d_grad), static_cast<O *>(d_table_grad), a);
+        const cudaError_t e = launch(grad_join_kernel<T, O, V>, join + zero, 256, 0, s, true, static_cast<const T *>(d_grad), static_cast<O *>(d_table_grad), a);
         if (e != cudaSuccess || units == 0) return e;
         return launch(grad_fix_kernel<O, V>, ceil_div(units, 8), 256, 0, s, true, static_cast<O *>(d_table_grad), a, (uint32_t) units);
     };
@@ -1210,7 +1342,7 @@ int glide_dispatch_rows(glide_ctx *ctx, const void *d_rows, int row_type, uint64
             default: return run(Width<2>{});
         }
     };
-    if (pairs <= kFew) {
+    if (pairs <= kFewPairs) {
         ROWS_CUDA(with_bytes([&](auto b) {
             return launch(dispatch_small_kernel<decltype(b)::value>, count + 1, 256, (partitions + 1) * 4, s, false, from, row_stride * e, (uint32_t) count, words, d_choice, choices, partitions,
                           to, sorted_stride * e, d_position, d_map, d_segment_start);

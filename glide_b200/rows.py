@@ -119,9 +119,9 @@ def lookup_rows_grad(ctx: Context, d_grad: torch.Tensor, d_ids: torch.Tensor, nu
         _check_result(ctx, out, (num, dim), dtype or out.dtype)
     to, to_kind, to_stride = _matrix(ctx, "out", out)
     need = ctx.lib.glide_lookup_rows_grad_workspace(num, dim, count)
-    scratch = d_grad.new_empty(need, dtype=torch.uint8)
+    scratch = d_grad.new_empty(need, dtype=torch.uint8) if need else None   # few ids need none
     ctx.check(ctx.lib.glide_lookup_rows_grad(ctx.handle, grad, kind, stride, ids, count, scale, to, to_kind, num, dim, to_stride,
-                                             1 if accumulate else 0, scratch.data_ptr(), need, _stream(ctx)))
+                                             1 if accumulate else 0, scratch.data_ptr() if need else None, need, _stream(ctx)))
     return out
 
 

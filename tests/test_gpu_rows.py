@@ -164,7 +164,7 @@ def test_lookup_grad_runs_of_every_length(gpu_ctx, runs, dim):
     assert torch.equal(rows.lookup_rows_grad(gpu_ctx, grad, ids, len(runs)).double(), want)
 
 
-@pytest.mark.parametrize("count", [1, 2, 255, 256, 257, 2047, 2048, 2049, 8191, 8192, 8193, 70_000])
+@pytest.mark.parametrize("count", [1, 2, 255, 256, 257, 1023, 1024, 1025, 2047, 2048, 2049, 4095, 4096, 4097, 8191, 8192, 8193, 70_000, 140_000])
 @pytest.mark.parametrize("n", [1, 2, 255, 256, 2047, 2048, 65_536, 4_194_304, 4_194_305])
 def test_lookup_grad_sorts_every_size(gpu_ctx, count, n):
     ids = _ids((count,), n, 14, 0.05)
@@ -581,11 +581,11 @@ def test_c_entry_points_refuse_what_they_do_not_take(gpu_ctx):
     grad(BAD, n=0)
     grad(BAD, g=None)
     grad(BAD, out=None)
-    grad(BAD, wb=100)
-    grad(BAD, w=None)
+    grad(BAD, count=2000, gs=1, wb=100)        # few ids need no workspace, these do
+    grad(BAD, count=2000, gs=1, w=None)
     grad(BAD, w=W + 16)
     grad(BAD, out=X)
-    grad(BAD, w=Y)
+    grad(BAD, count=2000, gs=0, w=Y)
     grad(BAD, os=10)
     grad(BAD, n=1 << 32)
 
