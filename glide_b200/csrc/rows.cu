@@ -30,10 +30,16 @@ constexpr uint32_t kFew = 4096;             // items that are sorted by comparin
 constexpr uint32_t kFewPairs = 2048;        // pairs that dispatch_rows places and copies in one launch (2,000: 6 to 8 us, by tiles 8)
 constexpr uint32_t kFewIds = 1024;          // ids whose gradient takes one launch
 constexpr uint32_t kMaxPassBits = 11;       // digits of a pass
-constexpr uint32_t kMaxFusedTiles = 64;     // tiles whose counts every CTA of the second kernel adds up by itself
+constexpr uint32_t kMaxFusedCounts = 16384; // counts (tiles x buckets) that every CTA of the second kernel adds up by itself
 constexpr uint32_t kClearShare = 24u << 20; // bytes of a gradient that are cleared beside each launch of its sort
 
 // ---- rows as words ----------------------------------------------------------------------------------------
+// A kernel handles a row in pieces of V values, a word of up to 16 bytes of its input: as many as the addresses, strides and lengths of
+// all matrices are multiples of. Rows of an odd number of 16-bit values (or of bytes) would leave an access for each value. Where that
+// costs most (lookup_kernel, combine_kernel) they have a second form, kWhole = false: a piece is what falls into a word of the row
+// that is WRITTEN, so that full words are stored, and what is read lies in two words beside each other, which are shifted into one;
+// words that would reach beyond the matrix are read value by value. 1,001 bf16 a row, both ways: 40,000 rows looked up 55 and 42 us,
+// 20,000 x 4 combined 119 and 62; but dispatched 71 and 94, the gradient of combine 115 and 170: there the shifting costs more.
 template<int B> struct Word;
 template<> struct Word<16> { using type = uint4; };
 template<> struct Word<8> { using type = uint2; };
@@ -51,24 +57,72 @@ template<> __device__ __forceinline__ float from_float<float>(float x) { return 
 template<> __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
 template<> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
-// A word from or to global memory as ONE access: a plain dereference that is copied into values of T next is split into
-// accesses of T by the compiler (93 % L1 hits and a quarter of the bandwidth in combine_kernel).
-template<bool kWritten, typename W>
-__device__ __forceinline__ W get_word(const W *p) {
-    if constexpr (kWritten) return __ldcg(p);
-    else return __ldg(p);
+// Rows of a matrix in device memory, and its first and last address.
+template<typename T>
+struct Rows {
+    T *p;
+    uint64_t stride;   // in values
+    uint64_t begin, end;
+    __device__ __forceinline__ T *row(uint64_t r) const { return p + r * stride; }
+};
+
+// A piece that has been asked for. Nothing may look at it before all pieces that are to be in flight have been: a conversion beside a
+// load makes the load be waited for before the next (combine_kernel: 1.9 of 6.5 TB/s).
+template<typename T, int V, bool kWhole>
+struct Piece {
+    WordOf<T, V> a;
+    __device__ __forceinline__ WordOf<T, V> word() const { return a; }
+};
+template<typename T, int V>
+struct Piece<T, V, false> {
+    WordOf<T, V> a, b;
+    uint32_t shift;   // bytes of a that come before the piece
+    __device__ __forceinline__ WordOf<T, V> word() const {
+        if constexpr (sizeof(a) == 4) {
+            return __funnelshift_r(a, b, shift * 8);
+        } else {
+            uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int i = 0; i < 6; i++) w[i] = shift & 8u ? w[i + 2] : w[i];
+#pragma unroll
+            for (int i = 0; i < 5; i++) w[i] = shift & 4u ? w[i + 1] : w[i];
+            if constexpr (sizeof(T) < 4) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) w[i] = __funnelshift_r(w[i], w[i + 1], (shift & 3u) * 8);
+            }
+            return make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+};
+
+// Values start .. start + V - 1 of a row of m; zeros where the piece is not wanted. Values outside of the row are anything.
+// One access a word: a plain dereference is split into values by the compiler when they are taken apart next.
+template<int V, bool kWhole, typename T>
+__device__ __forceinline__ Piece<T, V, kWhole> fetch(const Rows<const T> &m, const T *row, int32_t start, uint32_t dim, bool wanted) {
+    using W = WordOf<T, V>;
+    Piece<T, V, kWhole> piece;
+    memset(&piece, 0, sizeof piece);
+    if constexpr (kWhole) {
+        if (wanted) piece.a = __ldg(reinterpret_cast<const W *>(row + start));
+    } else if (wanted) {
+        const uint64_t at = reinterpret_cast<uintptr_t>(row) + (int64_t) start * (int64_t) sizeof(T), from = at & ~(uint64_t) (sizeof(W) - 1);
+        const uint32_t shift = (uint32_t) (at - from);
+        if (from >= m.begin && from + (shift ? 2 : 1) * sizeof(W) <= m.end) {
+            piece.a = __ldg(reinterpret_cast<const W *>(from));
+            if (shift) piece.b = __ldg(reinterpret_cast<const W *>(from) + 1);
+            piece.shift = shift;
+        } else {   // at either end of the matrix
+            T t[V];
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                memset(&t[i], 0, sizeof t[i]);
+                if (start + i >= 0 && start + i < (int32_t) dim) t[i] = row[start + i];
+            }
+            memcpy(&piece.a, t, sizeof piece.a);
+        }
+    }
+    return piece;
 }
-// Zeros where the word is not wanted. The words of several rows are fetched before any of them is taken apart: with the
-// conversion inside the condition each load is waited for before the next (1.9 of 6.5 TB/s in combine_kernel).
-template<typename W, typename T>
-__device__ __forceinline__ W get_word_if(const T *p, bool wanted) {
-    W w;
-    memset(&w, 0, sizeof w);
-    if (wanted) w = __ldg(reinterpret_cast<const W *>(p));
-    return w;
-}
-template<typename W>
-__device__ __forceinline__ void put_word(W *p, const W &w) { __stcg(p, w); }
 
 template<typename T, int V>
 __device__ __forceinline__ void unpack(const WordOf<T, V> &w, float (&f)[V]) {
@@ -78,42 +132,54 @@ __device__ __forceinline__ void unpack(const WordOf<T, V> &w, float (&f)[V]) {
     for (int i = 0; i < V; i++) f[i] = to_float(t[i]);
 }
 
-// V values stored as T; fp32 values of wider groups go out in words of 16 bytes
-template<typename T, int V>
-__device__ __forceinline__ void store(T *p, const float (&f)[V]) {
-    if constexpr (sizeof(T) * V <= 16) {
-        T t[V];
+// The first value of piece c of a row that is written.
+template<int V, bool kWhole, typename O>
+__device__ __forceinline__ int32_t piece_start(const O *row, uint32_t c) {
+    if constexpr (kWhole) return (int32_t) (c * V);
+    else return (int32_t) (c * V) - (int32_t) ((reinterpret_cast<uintptr_t>(row) & 15u) / sizeof(O));
+}
+// Pieces of such a row, at most.
+template<int V, typename O> constexpr uint32_t pieces(bool whole, uint32_t dim) { return whole ? dim / V : (dim + V - 1 + 16 / (uint32_t) sizeof(O) - 1) / V; }
+
+// V values in words of 16 bytes at most.
+template<typename O, int V>
+__device__ __forceinline__ void store(O *p, const float (&f)[V]) {
+    constexpr int H = 16 / (int) sizeof(O) < V ? 16 / (int) sizeof(O) : V;
 #pragma unroll
-        for (int i = 0; i < V; i++) t[i] = from_float<T>(f[i]);
-        WordOf<T, V> w;
+    for (int h = 0; h < V; h += H) {
+        O t[H];
+#pragma unroll
+        for (int i = 0; i < H; i++) t[i] = from_float<O>(f[h + i]);
+        WordOf<O, H> w;
         memcpy(&w, t, sizeof w);
-        put_word(reinterpret_cast<WordOf<T, V> *>(p), w);
-    } else {
-        constexpr int H = 16 / (int) sizeof(T);
+        __stcg(reinterpret_cast<WordOf<O, H> *>(p + h), w);
+    }
+}
+// kWritten: the memory is written in the same launch, each word by the thread that reads it
+template<typename O, int V, bool kWritten = false>
+__device__ __forceinline__ void load(const O *p, float (&f)[V]) {
+    constexpr int H = 16 / (int) sizeof(O) < V ? 16 / (int) sizeof(O) : V;
 #pragma unroll
-        for (int h = 0; h < V / H; h++) {
-            float g[H];
+    for (int h = 0; h < V; h += H) {
+        const auto *from = reinterpret_cast<const WordOf<O, H> *>(p + h);
+        const WordOf<O, H> w = kWritten ? __ldcg(from) : __ldg(from);
+        O t[H];
+        memcpy(t, &w, sizeof w);
 #pragma unroll
-            for (int i = 0; i < H; i++) g[i] = f[h * H + i];
-            store<T, H>(p + h * H, g);
-        }
+        for (int i = 0; i < H; i++) f[h + i] = to_float(t[i]);
     }
 }
 
-// kWritten: the memory is written in the same launch (each word by the thread that reads it)
-template<typename T, int V, bool kWritten = false>
-__device__ __forceinline__ void load(const T *p, float (&f)[V]) {
-    if constexpr (sizeof(T) * V <= 16) {
-        unpack<T, V>(get_word<kWritten>(reinterpret_cast<const WordOf<T, V> *>(p)), f);
+// A piece of a row that is written: the values of it that the row has.
+template<int V, bool kWhole, typename O>
+__device__ __forceinline__ void put(O *row, int32_t start, uint32_t dim, const float (&f)[V]) {
+    if (kWhole || (start >= 0 && start + V <= (int32_t) dim)) {
+        store<O, V>(row + start, f);
     } else {
-        constexpr int H = 16 / (int) sizeof(T);
+        const int32_t lo = -start, hi = (int32_t) dim - start;
 #pragma unroll
-        for (int h = 0; h < V / H; h++) {
-            float g[H];
-            load<T, H, kWritten>(p + h * H, g);
-#pragma unroll
-            for (int i = 0; i < H; i++) f[h * H + i] = g[i];
-        }
+        for (int i = 0; i < V; i++)
+            if (i >= lo && i < hi) row[start + i] = from_float<O>(f[i]);
     }
 }
 
@@ -129,32 +195,33 @@ struct Div {
 };
 
 // ---- lookup -------------------------------------------------------------------------------------------------
-// out[t] = scale * table[ids[t]], zeros for ids beyond the table (0xffffffff among them). A thread owns U words of the output, a
+// out[t] = scale * table[ids[t]], zeros for ids beyond the table (0xffffffff among them). A thread owns U pieces of the output, a
 // CTA's width apart, so that U loads are in flight once the ids (which a CTA shares through L1) have come.
-template<typename T, typename O, int V, int U>
-__global__ void __launch_bounds__(256) lookup_kernel(const T *__restrict__ table, uint64_t table_stride, uint32_t n,
-                                                     const uint32_t *__restrict__ ids, uint32_t units, Div words, float scale,
-                                                     O *__restrict__ out, uint64_t out_stride) {
+template<typename T, typename O, int V, bool kWhole, int U>
+__global__ void __launch_bounds__(256) lookup_kernel(Rows<const T> table, uint32_t n, uint32_t dim, const uint32_t *__restrict__ ids, uint32_t units, Div words,
+                                                     float scale, Rows<O> out) {
     const uint32_t first = blockIdx.x * (256 * U) + threadIdx.x;
-    uint32_t row[U], at[U], id[U];
+    uint32_t id[U];
+    int32_t at[U];
+    O *to[U];
+    Piece<T, V, kWhole> piece[U];
 #pragma unroll
     for (int u = 0; u < U; u++) {
-        const uint32_t x = min(first + u * 256, units - 1);
-        row[u] = words.of(x);
-        at[u] = (x - row[u] * words.d) * V;
-        id[u] = ids[row[u]];
+        const uint32_t x = min(first + u * 256, units - 1), row = words.of(x);
+        to[u] = out.row(row);
+        at[u] = piece_start<V, kWhole>(to[u], x - row * words.d);
+        id[u] = ids[row];
     }
-    WordOf<T, V> w[U];
 #pragma unroll
-    for (int u = 0; u < U; u++) w[u] = get_word_if<WordOf<T, V>>(table + (uint64_t) id[u] * table_stride + at[u], id[u] < n);
+    for (int u = 0; u < U; u++) piece[u] = fetch<V, kWhole>(table, table.row(id[u]), at[u], dim, id[u] < n);
 #pragma unroll
     for (int u = 0; u < U; u++) {
         if (first + u * 256 >= units) break;
         float f[V];
-        unpack<T, V>(w[u], f);
+        unpack<T, V>(piece[u].word(), f);
 #pragma unroll
-        for (int i = 0; i < V; i++) f[i] = id[u] < n ? f[i] * scale : 0.0f;
-        store<O, V>(out + (uint64_t) row[u] * out_stride + at[u], f);
+        for (int i = 0; i < V; i++) f[i] *= id[u] < n ? scale : 0.0f;   // what was not fetched is 0
+        put<V, kWhole>(to[u], at[u], dim, f);
     }
 }
 
@@ -191,8 +258,8 @@ cudaError_t launch(void (*kernel)(P...), uint64_t grid, uint32_t block, uint32_t
 // A CTA takes a tile of consecutive items, each of its warps a run of 256, 32 at a time: a lane's rank among the items of
 // its digit is the warp's running count plus the equal digits at lower lanes, and a scan over the warps' counts makes it the
 // rank in the tile. No atomics: the order depends on nothing but the keys. Few launches count most here (the data are 6 to 10
-// bytes an item): up to kFew items are sorted by one launch that compares each with all, up to kMaxFusedTiles tiles by two launches a
-// pass (every CTA of the second adds up the counts of all tiles), more by three. Tiles are small because their items' scattered stores leave an SM at
+// bytes an item): up to kFew items are sorted by one launch that compares each with all, more by two launches a pass while every CTA
+// of the second can add up the counts of all tiles, else by three. Tiles are small because their items' scattered stores leave an SM at
 // one sector a cycle: with 8,192 items to a tile a pass over 100,000 ids took 31 us.
 struct Digit {
     uint32_t limit, shift, bits;   // keys beyond limit count as limit; bits: of the digit
@@ -507,20 +574,18 @@ __global__ void __launch_bounds__(256) few_sort_kernel(const uint32_t *__restric
 // ---- gradient of a lookup ---------------------------------------------------------------------------------------
 struct GradArgs {
     const uint2 *sorted;             // by id: the id, and the row of the gradient
-    uint32_t items, n, dim, words, lanes, slabs, chunk;
+    uint32_t items, n, dim, words, lanes, slabs, chunk;   // words: pieces of a row
     float scale;
-    uint64_t in_stride, out_stride;
     int accumulate;
-    float *partial;                  // (2 * chunk + which) * dim: sums of runs that leave their chunk
-    uint64_t row_bytes;              // of the table's gradient, where its rows lie behind one another; otherwise 0
-    Div by_row_bytes;
+    float *partial;                  // at (2 * chunk + which) * dim: sums of runs that leave their chunk
+    Div by_row_bytes;                // of the table's gradient
     uint32_t join_blocks, clear_from, clear_rows;   // CTAs that join; the others clear clear_rows rows each, from row clear_from on
     __device__ __forceinline__ uint32_t key(uint64_t i) const { return sorted[i].x; }
 };
 
-template<typename O, int V>
-__device__ __forceinline__ void put_grad(O *out, const GradArgs &a, uint32_t id, uint32_t at, float (&acc)[V]) {
-    O *p = out + (uint64_t) id * a.out_stride + at;
+template<int V, typename O>
+__device__ __forceinline__ void put_grad(const Rows<O> &out, const GradArgs &a, uint32_t id, uint32_t word, float (&acc)[V]) {
+    O *p = out.row(id) + word * V;
 #pragma unroll
     for (int i = 0; i < V; i++) acc[i] *= a.scale;
     if (a.accumulate) {
@@ -569,72 +634,74 @@ __device__ __forceinline__ void name_rows(const GradArgs &a, uint32_t r0, uint32
 }
 
 // Rows [r0, r1) that `mark` does not name are cleared.
-template<typename O, int V, typename Mark>
-__device__ __forceinline__ void clear_rows(O *out, const GradArgs &a, uint32_t r0, uint32_t r1, Mark mark) {
+template<typename O, typename Mark>
+__device__ __forceinline__ void clear_rows(const Rows<O> &out, const GradArgs &a, uint32_t r0, uint32_t r1, Mark mark) {
     __shared__ uint32_t named[256 / 32];
     if (threadIdx.x < 8) named[threadIdx.x] = 0;
     __syncthreads();
     mark(named);
     __syncthreads();
-    if (a.row_bytes >= 16) {   // a word of 16 bytes lies in two rows at most; one that lies in a named and another one goes out in halves
-        uint8_t *at_bytes = reinterpret_cast<uint8_t *>(out) + r0 * a.row_bytes;
+    uint8_t *at = reinterpret_cast<uint8_t *>(out.row(r0));
+    const uint64_t row_bytes = (uint64_t) a.dim * sizeof(O);
+    if (out.stride == a.dim && row_bytes >= 16) {   // a word of 16 bytes lies in two rows at most; one that lies in a named and another one goes out in halves
         const auto is_named = [&](uint32_t byte) {
             const uint32_t r = a.by_row_bytes.of(byte);
             return (named[r >> 5] >> (r & 31u) & 1u) != 0;
         };
-        return clear_bytes(at_bytes, 0, (r1 - r0) * a.row_bytes, [&](uint32_t first, uint32_t last) {
+        clear_bytes(at, 0, (r1 - r0) * row_bytes, [&](uint32_t first, uint32_t last) {
             const bool x = is_named(first), y = is_named(last);
             if (x != y)
                 for (uint32_t o = first; o < last; o += 2)
-                    if (!is_named(o)) *reinterpret_cast<uint16_t *>(at_bytes + o) = 0;
+                    if (!is_named(o)) *reinterpret_cast<uint16_t *>(at + o) = 0;
             return x || y;
         });
-    }
-    float zero[V];
-#pragma unroll
-    for (int i = 0; i < V; i++) zero[i] = 0.0f;
-    for (uint32_t x = threadIdx.x; x < (r1 - r0) * a.words; x += blockDim.x) {
-        const uint32_t r = x / a.words, w = x - r * a.words;
-        if (!(named[r >> 5] >> (r & 31u) & 1u)) store<O, V>(out + (uint64_t) (r0 + r) * a.out_stride + w * V, zero);
+    } else if (row_bytes >= 256) {
+        for (uint32_t r = 0; r < r1 - r0; r++)
+            if (!(named[r >> 5] >> (r & 31u) & 1u)) clear_bytes(at + r * out.stride * sizeof(O), 0, row_bytes, [](uint32_t, uint32_t) { return false; });
+    } else {
+        for (uint32_t x = threadIdx.x; x < (r1 - r0) * a.dim; x += blockDim.x) {
+            const uint32_t r = x / a.dim;
+            if (!(named[r >> 5] >> (r & 31u) & 1u)) out.row(r0 + r)[x - r * a.dim] = from_float<O>(0.0f);
+        }
     }
 }
 
 // A group of lanes joins a chunk of sorted items over a slab of the row: the sum of a run of equal ids goes to the id's row, or,
 // where the run goes on in another chunk, to the chunk's partial sums (first: it came from the chunk before).
 template<typename T, typename O, int V>
-__global__ void __launch_bounds__(256, 4) grad_join_kernel(const T *__restrict__ grad, O *__restrict__ out, GradArgs a) {
+__global__ void __launch_bounds__(256, 4) grad_join_kernel(Rows<const T> grad, Rows<O> out, GradArgs a) {
     constexpr int U = 4;
     wait_for_previous();
     if (blockIdx.x >= a.join_blocks) {
         const uint64_t r0 = a.clear_from + (uint64_t) (blockIdx.x - a.join_blocks) * a.clear_rows;
         const uint32_t r1 = (uint32_t) min((uint64_t) a.n, r0 + a.clear_rows);
-        return clear_rows<O, V>(out, a, (uint32_t) r0, r1, [&](uint32_t *named) { name_rows(a, (uint32_t) r0, r1, named); });
+        return clear_rows(out, a, (uint32_t) r0, r1, [&](uint32_t *named) { name_rows(a, (uint32_t) r0, r1, named); });
     }
     const uint32_t group = (blockIdx.x * 256 + threadIdx.x) / a.lanes, lane = threadIdx.x & (a.lanes - 1);
     const uint32_t chunk = group / a.slabs, word = (group - chunk * a.slabs) * a.lanes + lane;
     const uint64_t c0 = (uint64_t) chunk * a.chunk;
     if (c0 >= a.items || word >= a.words) return;
-    const uint32_t c1 = (uint32_t) min(c0 + a.chunk, (uint64_t) a.items), at = word * V;
+    const uint32_t c1 = (uint32_t) min(c0 + a.chunk, (uint64_t) a.items);
     uint32_t id = a.key(c0);
     bool from_left = c0 > 0 && a.key(c0 - 1) == id;
     float acc[V];
 #pragma unroll
     for (int i = 0; i < V; i++) acc[i] = 0.0f;
-    auto put = [&](bool to_right) {
+    auto leave = [&](bool to_right) {
         if (id >= a.n) return;
-        if (from_left || to_right) store<float, V>(a.partial + (2ull * chunk + (from_left ? 0 : 1)) * a.dim + at, acc);
-        else put_grad<O, V>(out, a, id, at, acc);
+        if (from_left || to_right) store<float, V>(a.partial + (2ull * chunk + (from_left ? 0 : 1)) * a.dim + word * V, acc);
+        else put_grad<V>(out, a, id, word, acc);
     };
     uint2 next[U];   // items of the batch to come: their rows can be fetched without waiting for them
 #pragma unroll
     for (int u = 0; u < U; u++) next[u] = __ldg(a.sorted + min((uint32_t) c0 + u, c1 - 1));
     for (uint32_t c = (uint32_t) c0; c < c1; c += U) {
         uint32_t key[U];
-        WordOf<T, V> w[U];
+        Piece<T, V, true> piece[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
             key[u] = next[u].x;
-            w[u] = get_word_if<WordOf<T, V>>(grad + (uint64_t) next[u].y * a.in_stride + at, key[u] < a.n && c + u < c1);
+            piece[u] = fetch<V, true>(grad, grad.row(next[u].y), (int32_t) (word * V), a.dim, key[u] < a.n && c + u < c1);
         }
 #pragma unroll
         for (int u = 0; u < U; u++) next[u] = __ldg(a.sorted + min(c + U + u, c1 - 1));
@@ -642,7 +709,7 @@ __global__ void __launch_bounds__(256, 4) grad_join_kernel(const T *__restrict__
         for (int u = 0; u < U; u++) {
             if (c + u >= c1) break;
             if (key[u] != id) {
-                put(false);
+                leave(false);
                 id = key[u];
                 from_left = false;
 #pragma unroll
@@ -650,20 +717,20 @@ __global__ void __launch_bounds__(256, 4) grad_join_kernel(const T *__restrict__
             }
             if (id < a.n) {
                 float f[V];
-                unpack<T, V>(w[u], f);
+                unpack<T, V>(piece[u].word(), f);
 #pragma unroll
                 for (int i = 0; i < V; i++) acc[i] += f[i];
             }
         }
     }
-    put(c1 < a.items && a.key(c1) == id);
+    leave(c1 < a.items && a.key(c1) == id);
 }
 
 // Few ids: everything in one launch. A CTA owns one id, unless an earlier one is equal: it lists the equal ones in order, its groups of
 // lanes add consecutive parts of the list and the groups' sums are added in order. The other CTAs clear the rows that no id names.
-// 1,000 ids: see the table of kFewIds below. An id that is most of them is one CTA's work: at worst, 1,024 equal ids of 8 KB rows, 60 us.
+// Rows of 64 bf16: 10 ids 3.0 us, 1,000 ids 7.5, against 7.3 and 10.5 by three launches.
 template<typename T, typename O, int V>
-__global__ void __launch_bounds__(256) grad_few_kernel(const T *__restrict__ grad, O *__restrict__ out, const uint32_t *__restrict__ ids, GradArgs a) {
+__global__ void __launch_bounds__(256) grad_few_kernel(Rows<const T> grad, Rows<O> out, const uint32_t *__restrict__ ids, GradArgs a) {
     constexpr int U = 8;
     __shared__ uint32_t keys[kFewIds], counts[8];
     __shared__ uint16_t list[kFewIds];
@@ -673,7 +740,7 @@ __global__ void __launch_bounds__(256) grad_few_kernel(const T *__restrict__ gra
     if (blockIdx.x >= a.items) {
         const uint64_t r0 = (uint64_t) (blockIdx.x - a.items) * a.clear_rows;
         const uint32_t r1 = (uint32_t) min((uint64_t) a.n, r0 + a.clear_rows);
-        return clear_rows<O, V>(out, a, (uint32_t) r0, r1, [&](uint32_t *named) {
+        return clear_rows(out, a, (uint32_t) r0, r1, [&](uint32_t *named) {
             for (uint32_t i = threadIdx.x; i < a.items; i += 256)
                 if (keys[i] >= r0 && keys[i] < r1) atomicOr(&named[(keys[i] - (uint32_t) r0) >> 5], 1u << ((keys[i] - (uint32_t) r0) & 31u));
         });
@@ -707,20 +774,20 @@ __global__ void __launch_bounds__(256) grad_few_kernel(const T *__restrict__ gra
 #pragma unroll
         for (int i = 0; i < V; i++) acc[i] = 0.0f;
         for (uint32_t s = s0; s < s1; s += U) {
-            WordOf<T, V> w[U];
+            Piece<T, V, true> piece[U];
 #pragma unroll
-            for (int u = 0; u < U; u++) w[u] = get_word_if<WordOf<T, V>>(grad + (uint64_t) list[min(s + u, s1 - 1)] * a.in_stride + word * V, s + u < s1);
+            for (int u = 0; u < U; u++) piece[u] = fetch<V, true>(grad, grad.row(list[min(s + u, s1 - 1)]), (int32_t) (word * V), a.dim, s + u < s1);
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 if (s + u >= s1) break;
                 float f[V];
-                unpack<T, V>(w[u], f);
+                unpack<T, V>(piece[u].word(), f);
 #pragma unroll
                 for (int i = 0; i < V; i++) acc[i] += f[i];
             }
         }
         if (groups == 1) {
-            put_grad<O, V>(out, a, id, word * V, acc);
+            put_grad<V>(out, a, id, word, acc);
         } else {
 #pragma unroll
             for (int i = 0; i < V; i++) part[threadIdx.x][i] = acc[i];
@@ -736,7 +803,7 @@ __global__ void __launch_bounds__(256) grad_few_kernel(const T *__restrict__ gra
     for (uint32_t g = 1; g < used; g++)
 #pragma unroll
         for (int i = 0; i < V; i++) acc[i] += part[g * a.lanes + threadIdx.x][i];
-    put_grad<O, V>(out, a, id, threadIdx.x * V, acc);
+    put_grad<V>(out, a, id, threadIdx.x, acc);
 }
 
 // Runs over several chunks, whose first chunk's unit (a chunk and a slab) adds their partial sums and writes the row. A warp owns a unit and
@@ -744,18 +811,18 @@ __global__ void __launch_bounds__(256) grad_few_kernel(const T *__restrict__ gra
 // and the warps' sums are added in order.
 constexpr uint32_t kLongRun = 32;
 template<typename O, int V>
-__global__ void __launch_bounds__(256) grad_fix_kernel(O *__restrict__ out, GradArgs a, uint32_t units) {
+__global__ void __launch_bounds__(256) grad_fix_kernel(Rows<O> out, GradArgs a, uint32_t units) {
     __shared__ float part[8][32][V];
     __shared__ uint32_t long_last[8];
     wait_for_previous();
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-    auto add = [&](uint32_t chunk, uint32_t at, uint32_t s0, uint32_t s1, float (&acc)[V]) {   // partial sums s0 .. s1 - 1 of the run that starts in chunk
+    auto add = [&](uint32_t chunk, uint32_t word, uint32_t s0, uint32_t s1, float (&acc)[V]) {   // partial sums s0 .. s1 - 1 of the run that starts in chunk
 #pragma unroll
         for (int i = 0; i < V; i++) acc[i] = 0.0f;
 #pragma unroll 8
         for (uint32_t s = s0; s < s1; s++) {
             float f[V];
-            load<float, V>(a.partial + (2ull * (chunk + s) + (s == 0 ? 1 : 0)) * a.dim + at, f);
+            load<float, V>(a.partial + (2ull * (chunk + s) + (s == 0 ? 1 : 0)) * a.dim + word * V, f);
 #pragma unroll
             for (int i = 0; i < V; i++) acc[i] += f[i];
         }
@@ -780,8 +847,8 @@ __global__ void __launch_bounds__(256) grad_fix_kernel(O *__restrict__ out, Grad
             }
             if (last - chunk < kLongRun && lane < a.lanes && word < a.words) {
                 float acc[V];
-                add(chunk, word * V, 0, last - chunk + 1, acc);
-                put_grad<O, V>(out, a, id, word * V, acc);
+                add(chunk, word, 0, last - chunk + 1, acc);
+                put_grad<V>(out, a, id, word, acc);
             }
             if (last - chunk < kLongRun) last = 0;
         }
@@ -802,7 +869,7 @@ __global__ void __launch_bounds__(256) grad_fix_kernel(O *__restrict__ out, Grad
         const bool mine = there && lane < a.lanes && word < a.words;
         float acc[V];
         if (mine) {
-            add(chunk, word * V, s0, s1, acc);
+            add(chunk, word, s0, s1, acc);
 #pragma unroll
             for (int i = 0; i < V; i++) part[warp][lane][i] = acc[i];
         }
@@ -811,7 +878,7 @@ __global__ void __launch_bounds__(256) grad_fix_kernel(O *__restrict__ out, Grad
             for (uint32_t w = 1; w < each; w++)
 #pragma unroll
                 for (int i = 0; i < V; i++) acc[i] += part[warp + w][lane][i];
-            put_grad<O, V>(out, a, a.key((uint64_t) (chunk + 1) * a.chunk - 1), word * V, acc);
+            put_grad<V>(out, a, a.key((uint64_t) (chunk + 1) * a.chunk - 1), word, acc);
         }
         __syncthreads();
     }
@@ -819,19 +886,18 @@ __global__ void __launch_bounds__(256) grad_fix_kernel(O *__restrict__ out, Grad
 
 // ---- dispatch ---------------------------------------------------------------------------------------------------
 // Each row, read once, is copied to the places of its pairs. A thread has U words of rows in flight.
-template<int B, int U>
-__global__ void __launch_bounds__(256) dispatch_kernel(const uint8_t *__restrict__ rows, uint64_t stride, uint32_t units, Div words, uint32_t choices,
-                                                       const uint32_t *__restrict__ position, uint8_t *__restrict__ sorted, uint64_t sorted_stride) {
-    using W = typename Word<B>::type;
+template<typename T, int V, int U>
+__global__ void __launch_bounds__(256) dispatch_kernel(Rows<const T> rows, uint32_t dim, uint32_t units, Div words, uint32_t choices,
+                                                       const uint32_t *__restrict__ position, Rows<T> sorted) {
     const uint32_t first = blockIdx.x * (256 * U) + threadIdx.x;
     uint32_t row[U], at[U];
-    W w[U];
+    Piece<T, V, true> piece[U];
 #pragma unroll
     for (int u = 0; u < U; u++) {
         const uint32_t x = min(first + u * 256, units - 1);
         row[u] = words.of(x);
-        at[u] = (x - row[u] * words.d) * B;
-        w[u] = get_word<false>(reinterpret_cast<const W *>(rows + (uint64_t) row[u] * stride + at[u]));
+        at[u] = (x - row[u] * words.d) * V;
+        piece[u] = fetch<V, true>(rows, rows.row(row[u]), (int32_t) at[u], dim, true);
     }
     wait_for_previous();   // the places come from the launch before, the rows do not
 #pragma unroll
@@ -840,19 +906,17 @@ __global__ void __launch_bounds__(256) dispatch_kernel(const uint8_t *__restrict
 #pragma unroll 4
         for (uint32_t j = 0; j < choices; j++) {
             const uint32_t p = position[(uint64_t) row[u] * choices + j];
-            if (p != kNone) put_word(reinterpret_cast<W *>(sorted + (uint64_t) p * sorted_stride + at[u]), w[u]);
+            if (p != kNone) __stcg(reinterpret_cast<WordOf<T, V> *>(sorted.row(p) + at[u]), piece[u].a);
         }
     }
 }
 
 // Few pairs: everything in one launch. A CTA owns one row; a warp finds a pair's place by comparing it with all pairs, then the CTA
 // copies the row. One CTA more counts the partitions.
-template<int B>
-__global__ void __launch_bounds__(256) dispatch_small_kernel(const uint8_t *__restrict__ rows, uint64_t stride, uint32_t count, uint32_t words,
-                                                             const uint32_t *__restrict__ choice, uint32_t choices, uint32_t partitions,
-                                                             uint8_t *__restrict__ sorted, uint64_t sorted_stride, uint32_t *__restrict__ position,
-                                                             uint32_t *__restrict__ map, uint32_t *__restrict__ segment_start) {
-    using W = typename Word<B>::type;
+template<typename T, int V>
+__global__ void __launch_bounds__(256) dispatch_small_kernel(Rows<const T> rows, uint32_t dim, uint32_t count, uint32_t words,
+                                                             const uint32_t *__restrict__ choice, uint32_t choices, uint32_t partitions, Rows<T> sorted,
+                                                             uint32_t *__restrict__ position, uint32_t *__restrict__ map, uint32_t *__restrict__ segment_start) {
     __shared__ uint4 all[kFewPairs / 4];
     __shared__ uint32_t place[kMaxChoices];
     extern __shared__ __align__(16) uint32_t counts[];
@@ -869,10 +933,9 @@ __global__ void __launch_bounds__(256) dispatch_small_kernel(const uint8_t *__re
         return;
     }
     few_keys(choice, pairs, partitions, all);
-    W w;
-    memset(&w, 0, sizeof w);
-    const uint8_t *from = rows + (uint64_t) row * stride;
-    if (threadIdx.x < words) w = get_word<false>(reinterpret_cast<const W *>(from + (uint64_t) threadIdx.x * B));
+    const T *from = rows.row(row);
+    Piece<T, V, true> piece{};   // fetched before the places are known
+    if (threadIdx.x < words) piece = fetch<V, true>(rows, from, (int32_t) (threadIdx.x * V), dim, true);
     __syncthreads();
     for (uint32_t j = warp; j < choices; j += 8) {
         const uint32_t pair = row * choices + j, key = reinterpret_cast<const uint32_t *>(all)[pair], before = few_place(all, pairs, pair, key);
@@ -884,31 +947,29 @@ __global__ void __launch_bounds__(256) dispatch_small_kernel(const uint8_t *__re
     }
     __syncthreads();
     for (uint32_t c = threadIdx.x; c < words; c += 256) {
-        if (c != threadIdx.x) w = get_word<false>(reinterpret_cast<const W *>(from + (uint64_t) c * B));
-        for (uint32_t j = 0; j < choices; j++) {
-            const uint32_t p = place[j];
-            if (p != kNone) put_word(reinterpret_cast<W *>(sorted + (uint64_t) p * sorted_stride + (uint64_t) c * B), w);
-        }
+        if (c != threadIdx.x) piece = fetch<V, true>(rows, from, (int32_t) (c * V), dim, true);
+        for (uint32_t j = 0; j < choices; j++)
+            if (place[j] != kNone) __stcg(reinterpret_cast<WordOf<T, V> *>(sorted.row(place[j]) + c * V), piece.a);
     }
 }
 
 // ---- combine ----------------------------------------------------------------------------------------------------
-// out[t] = sum over j, ascending, of weight[t,j] * sorted[position[t,j]]; K pairs' words are in flight for each word of a row.
-template<typename T, int V, int K>
-__global__ void __launch_bounds__(256) combine_kernel(const T *__restrict__ sorted, uint64_t stride, uint32_t sorted_rows,
-                                                      const uint32_t *__restrict__ position, uint32_t choices,
-                                                      const float *__restrict__ weights, uint32_t units, Div words, T *__restrict__ out,
-                                                      uint64_t out_stride) {
+// out[t] = sum over j, ascending, of weight[t,j] * sorted[position[t,j]]; K pairs' pieces are in flight for each piece of a row.
+template<typename T, int V, bool kWhole, int K>
+__global__ void __launch_bounds__(256) combine_kernel(Rows<const T> sorted, uint32_t sorted_rows, uint32_t dim, const uint32_t *__restrict__ position,
+                                                      uint32_t choices, const float *__restrict__ weights, uint32_t units, Div words, Rows<T> out) {
     const uint32_t x = blockIdx.x * 256 + threadIdx.x;
     if (x >= units) return;
-    const uint32_t row = words.of(x), at = (x - row * words.d) * V;
+    const uint32_t row = words.of(x);
+    T *to = out.row(row);
+    const int32_t at = piece_start<V, kWhole>(to, x - row * words.d);
     float acc[V];
 #pragma unroll
     for (int i = 0; i < V; i++) acc[i] = 0.0f;
     for (uint32_t j0 = 0; j0 < choices; j0 += K) {
         uint32_t p[K];
         float w[K];
-        WordOf<T, V> y[K];
+        Piece<T, V, kWhole> y[K];
 #pragma unroll
         for (int j = 0; j < K; j++) {
             const uint64_t pair = (uint64_t) row * choices + j0 + j;
@@ -916,31 +977,30 @@ __global__ void __launch_bounds__(256) combine_kernel(const T *__restrict__ sort
             w[j] = weights && j0 + j < choices ? weights[pair] : 1.0f;
         }
 #pragma unroll
-        for (int j = 0; j < K; j++) y[j] = get_word_if<WordOf<T, V>>(sorted + (uint64_t) p[j] * stride + at, p[j] < sorted_rows);
+        for (int j = 0; j < K; j++) y[j] = fetch<V, kWhole>(sorted, sorted.row(p[j]), at, dim, p[j] < sorted_rows);
 #pragma unroll
         for (int j = 0; j < K; j++) {
             if (p[j] >= sorted_rows) continue;
             float f[V];
-            unpack<T, V>(y[j], f);
+            unpack<T, V>(y[j].word(), f);
 #pragma unroll
             for (int i = 0; i < V; i++) acc[i] = fmaf(w[j], f[i], acc[i]);
         }
     }
-    store<T, V>(out + (uint64_t) row * out_stride + at, acc);
+    put<V, kWhole>(to, at, dim, acc);
 }
 
 // grad_sorted[position[t,j]] = weight[t,j] * grad[t] and grad_weights[t,j] = <grad[t], sorted[position[t,j]]>: G lanes own a row,
-// and have U of its words and those of K of its places in flight. A warp a row beats a CTA a row (16,384 x 8 rows of 4 KB: 180 against
+// and have U of its pieces and those of K of its places in flight. A warp a row beats a CTA a row (16,384 x 8 rows of 4 KB: 180 against
 // 205 us; 39,047 x 4 of 5 KB: 278 against 340) but where rows are few (64 x 8: 9.1 against 3.3; 1,000 x 4 of 8 KB: 22 against 16).
 template<typename T, int V, int K, int U, int G>
-__global__ void __launch_bounds__(256) combine_grad_kernel(const T *__restrict__ grad, uint64_t grad_stride, uint32_t count, uint32_t words,
-                                                           const T *__restrict__ sorted, uint64_t stride, uint32_t sorted_rows,
-                                                           const uint32_t *__restrict__ position, uint32_t choices,
-                                                           const float *__restrict__ weights, T *__restrict__ grad_sorted,
-                                                           uint64_t grad_sorted_stride, float *__restrict__ grad_weights) {
+__global__ void __launch_bounds__(256) combine_grad_kernel(Rows<const T> grad, uint32_t count, uint32_t dim, uint32_t words, Rows<const T> sorted, uint32_t sorted_rows,
+                                                           const uint32_t *__restrict__ position, uint32_t choices, const float *__restrict__ weights,
+                                                           Rows<T> grad_sorted, float *__restrict__ grad_weights) {
     __shared__ float part[8][K];
     const uint32_t row = blockIdx.x * (256 / G) + threadIdx.x / G, l = threadIdx.x % G;
     if (G == 32 && row >= count) return;
+    const T *from = grad.row(row);
     for (uint32_t j0 = 0; j0 < choices; j0 += K) {
         uint32_t p[K];
         float w[K], dot[K];
@@ -952,32 +1012,32 @@ __global__ void __launch_bounds__(256) combine_grad_kernel(const T *__restrict__
             dot[j] = 0.0f;
         }
         for (uint32_t c0 = l; c0 < words; c0 += G * U) {
-            WordOf<T, V> x[U], y[U][K];
+            Piece<T, V, true> x[U], y[U][K];
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 const uint32_t c = c0 + u * G;
                 const bool in = u == 0 || c < words;
-                x[u] = get_word_if<WordOf<T, V>>(grad + (uint64_t) row * grad_stride + (uint64_t) c * V, in);
+                x[u] = fetch<V, true>(grad, from, (int32_t) (c * V), dim, in);
 #pragma unroll
-                for (int j = 0; j < K; j++) y[u][j] = get_word_if<WordOf<T, V>>(sorted + (uint64_t) p[j] * stride + (uint64_t) c * V, in && p[j] < sorted_rows);
+                for (int j = 0; j < K; j++) y[u][j] = fetch<V, true>(sorted, sorted.row(p[j]), (int32_t) (c * V), dim, in && p[j] < sorted_rows);
             }
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 const uint32_t c = c0 + u * G;
                 if (u > 0 && c >= words) break;
                 float g[V];
-                unpack<T, V>(x[u], g);
+                unpack<T, V>(x[u].word(), g);
 #pragma unroll
                 for (int j = 0; j < K; j++) {
                     if (p[j] >= sorted_rows) continue;
                     float f[V], o[V];
-                    unpack<T, V>(y[u][j], f);
+                    unpack<T, V>(y[u][j].word(), f);
 #pragma unroll
                     for (int i = 0; i < V; i++) {
                         dot[j] = fmaf(g[i], f[i], dot[j]);
                         o[i] = w[j] * g[i];
                     }
-                    store<T, V>(grad_sorted + (uint64_t) p[j] * grad_sorted_stride + (uint64_t) c * V, o);
+                    store<T, V>(grad_sorted.row(p[j]) + c * V, o);
                 }
             }
         }
@@ -1039,9 +1099,9 @@ struct OnDevice {
     ~OnDevice() { if (before >= 0) cudaSetDevice(before); }
 };
 
-#define ROWS_CUDA(call)                                                                                      \
+#define ROWS_CUDA(...)                                                                                      \
     do {                                                                                                     \
-        const cudaError_t e_ = (call);                                                                       \
+        const cudaError_t e_ = (__VA_ARGS__);                                                                     \
         if (e_ != cudaSuccess) return fail(ctx, GLIDE_ERR_CUDA, "%s: %s", __func__, cudaGetErrorString(e_)); \
     } while (0)
 
@@ -1056,13 +1116,18 @@ struct Matrix {
     int type;
     uint64_t bytes() const { return rows == 0 ? 0 : ((rows - 1) * stride + dim) * bytes_of(type); }
     bool sized() const { return stride <= (1ull << 40) && rows <= (1ull << 32); }
-    // The most values (a power of two up to `most`) that a word may hold so that every word of every row is aligned.
+    // The most values (1, 2, 4 or 8) that a word may hold so that every word of every row is aligned, words of 16 bytes at most.
     uint32_t width(uint32_t most) const {
-        const uint32_t e = bytes_of(type);
+        const uint64_t e = bytes_of(type);
         uint32_t v = most;
-        while (v > 1 && (reinterpret_cast<uintptr_t>(p) % (v * e) || (rows > 1 && stride % v) || dim % v)) v >>= 1;
+        for (; v > 1; v >>= 1) {
+            const uint64_t word = v * e < 16 ? v * e : 16;
+            if (reinterpret_cast<uintptr_t>(p) % word == 0 && (rows <= 1 || stride * e % word == 0) && dim % v == 0) break;
+        }
         return v;
     }
+    template<typename T> Rows<T> as() const { return Rows<T>{static_cast<T *>(const_cast<void *>(p)), stride, reinterpret_cast<uintptr_t>(p), reinterpret_cast<uintptr_t>(p) + bytes()}; }
+    Matrix from(uint64_t r) const { return Matrix{static_cast<const char *>(p) + r * stride * bytes_of(type), rows - r, stride, dim, type}; }
 };
 
 bool aligned(const Matrix &m) { return reinterpret_cast<uintptr_t>(m.p) % bytes_of(m.type) == 0; }
@@ -1075,39 +1140,55 @@ bool overlap(const Matrix &a, const Matrix &b) { return overlap(a.p, a.bytes(), 
 uint64_t align256(uint64_t x) { return (x + 255) & ~(uint64_t) 255; }
 uint64_t ceil_div(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
 
-// f(width as a constant) for a width of 1, 2, 4 or 8 values
-template<int V> struct Width { static constexpr int value = V; };
-template<int kMost, typename F> cudaError_t with_width(uint32_t v, F f) {
-    if constexpr (kMost >= 8) if (v >= 8) return f(Width<8>{});
-    if constexpr (kMost >= 4) if (v >= 4) return f(Width<4>{});
-    if (v >= 2) return f(Width<2>{});
-    return f(Width<1>{});
-}
+template<int N> struct Number { static constexpr int value = N; };
 
-// f(a value of the type, Width) for rows of floating types
+uint32_t values_of(int type) { return type == GLIDE_ROW_F32 || type == GLIDE_ROW_U8 ? 4 : 8; }   // of a piece, at most
+uint32_t min_of(uint32_t a, uint32_t b) { return a < b ? a : b; }
+
+// f(the width as a constant)
+template<int kMost, typename F> cudaError_t with_width(uint32_t v, F f) {
+    if constexpr (kMost >= 8) if (v >= 8) return f(Number<8>{});
+    if (v >= 4) return f(Number<4>{});
+    if (v >= 2) return f(Number<2>{});
+    return f(Number<1>{});
+}
+// f(a value of the type, the width) for rows of floating types
 template<typename F> cudaError_t with_rows(int type, uint32_t v, F f) {
     if (type == GLIDE_ROW_F32) return with_width<4>(v, [&](auto w) { return f(float{}, w); });
     if (type == GLIDE_ROW_F16) return with_width<8>(v, [&](auto w) { return f(__half{}, w); });
     return with_width<8>(v, [&](auto w) { return f(__nv_bfloat16{}, w); });
 }
-uint32_t most_of(int type) { return type == GLIDE_ROW_F32 || type == GLIDE_ROW_U8 ? 4 : 8; }
+// f(a value of the type, the width, whether rows are whole words): 16-bit values that would go one by one are shifted instead
+template<typename F> cudaError_t with_rows_or_shifted(int type, uint32_t v, F f) {
+    return with_rows(type, type != GLIDE_ROW_F32 && v == 1 ? 8 : v, [&](auto t, auto w) {
+        if constexpr (sizeof t == 2 && decltype(w)::value == 8)
+            if (v == 1) return f(t, w, Number<0>{});
+        if constexpr (sizeof t == 2 && decltype(w)::value == 1) return cudaErrorInvalidValue;   // the shifted form takes these
+        else return f(t, w, Number<1>{});
+    });
+}
 
-template<typename T, typename O, int V>
-cudaError_t launch_lookup(const void *table, uint64_t table_stride, uint32_t n, const uint32_t *ids, uint64_t count, uint32_t dim, float scale,
-                          void *out, uint64_t out_stride, cudaStream_t stream) {
-    const uint32_t words = dim / V;
-    const uint64_t most = 0x7fff0000u / words;   // rows of a launch: its words are counted in 31 bits
-    for (uint64_t r0 = 0; r0 < count; r0 += most) {
-        const uint32_t rows = (uint32_t) (count - r0 < most ? count - r0 : most), units = rows * words;
-        O *to = static_cast<O *>(out) + r0 * out_stride;
-        if (units <= 256 * 1024)
-            lookup_kernel<T, O, V, 1><<<(uint32_t) ceil_div(units, 256), 256, 0, stream>>>(static_cast<const T *>(table), table_stride, n, ids + r0, units, Div(words), scale, to, out_stride);
-        else
-            lookup_kernel<T, O, V, 4><<<(uint32_t) ceil_div(units, 1024), 256, 0, stream>>>(static_cast<const T *>(table), table_stride, n, ids + r0, units, Div(words), scale, to, out_stride);
-        const cudaError_t e = cudaGetLastError();
+// f(first row, rows) for parts of a call whose pieces a launch can count in 31 bits
+template<typename F> cudaError_t in_parts(uint64_t count, uint32_t words, F f) {
+    const uint64_t each = 0x7fff0000u / words;
+    for (uint64_t r0 = 0; r0 < count; r0 += each) {
+        const cudaError_t e = f(r0, (uint32_t) (count - r0 < each ? count - r0 : each));
         if (e != cudaSuccess) return e;
     }
     return cudaSuccess;
+}
+
+template<typename T, typename O, int V, bool kWhole>
+cudaError_t launch_lookup(const Matrix &table, const uint32_t *ids, float scale, const Matrix &out, cudaStream_t stream) {
+    const uint32_t words = pieces<V, O>(kWhole, out.dim);
+    return in_parts(out.rows, words, [&](uint64_t r0, uint32_t rows) {
+        const uint32_t units = rows * words;
+        auto go = [&](auto u) {
+            return launch(lookup_kernel<T, O, V, kWhole, decltype(u)::value>, ceil_div(units, 256 * decltype(u)::value), 256, 0, stream, false, table.as<const T>(), (uint32_t) table.rows,
+                          out.dim, ids + r0, units, Div(words), scale, out.from(r0).as<O>());
+        };
+        return units <= 256 * 1024 ? go(Number<1>{}) : go(Number<4>{});
+    });
 }
 
 uint32_t bits_for(uint64_t values) {   // to write 0 .. values - 1
@@ -1125,7 +1206,7 @@ cudaError_t sort_pass(const Keys &keys, uint32_t items, const Digit &digit, uint
     cudaError_t e = launch(bucket_count_kernel, tiles + c.blocks(), kTileThreads, rank_smem(kTileThreads / 32, buckets), stream, dependent, keys, items, digit, buckets, tiles, counts, ranks, c);
     if (e != cudaSuccess) return e;
     c = clear();
-    if (tiles <= kMaxFusedTiles)
+    if ((uint64_t) tiles * count_stride(buckets) <= kMaxFusedCounts)
         return launch(bucket_place_kernel<To, false>, tiles + c.blocks(), kTileThreads, count_stride(buckets) * 8, stream, true, keys, items, digit, buckets, tiles, counts, totals, ranks, to, c);
     e = launch(bucket_scan_kernel, ceil_div(buckets, 32), 1024, 0, stream, true, counts, tiles, buckets, totals);
     if (e != cudaSuccess) return e;
@@ -1202,12 +1283,12 @@ int glide_lookup_rows(glide_ctx *ctx, const void *d_table, int row_type, uint64_
     ROWS_REQUIRE(!overlap(out, table) && !overlap(d_out, out.bytes(), d_ids, count * 4), GLIDE_ERR_BAD_ARG, "lookup_rows: the result overlaps an input");
     const OnDevice guard(ctx->device);
     ROWS_CUDA(guard.status);
-    const uint32_t most = most_of(row_type), v0 = table.width(most), v1 = out.width(most), v = v0 < v1 ? v0 : v1;
+    const uint32_t most = values_of(row_type), v = min_of(table.width(most), out.width(most));
     auto s = static_cast<cudaStream_t>(stream);
-    if (row_type == GLIDE_ROW_U8)
-        ROWS_CUDA(with_width<4>(v, [&](auto w) { return launch_lookup<uint8_t, float, decltype(w)::value>(d_table, table_stride, (uint32_t) n, d_ids, count, dim, scale, d_out, out_stride, s); }));
-    else
-        ROWS_CUDA(with_rows(row_type, v, [&](auto t, auto w) { return launch_lookup<decltype(t), decltype(t), decltype(w)::value>(d_table, table_stride, (uint32_t) n, d_ids, count, dim, scale, d_out, out_stride, s); }));
+    if (row_type == GLIDE_ROW_U8) ROWS_CUDA(v == 4 ? launch_lookup<uint8_t, float, 4, true>(table, d_ids, scale, out, s) : launch_lookup<uint8_t, float, 4, false>(table, d_ids, scale, out, s));
+    else ROWS_CUDA(with_rows_or_shifted(row_type, v, [&](auto t, auto w, auto wh) {
+        return launch_lookup<decltype(t), decltype(t), decltype(w)::value, decltype(wh)::value != 0>(table, d_ids, scale, out, s);
+    }));
     return GLIDE_OK;
 }
 
@@ -1236,26 +1317,31 @@ int glide_lookup_rows_grad(glide_ctx *ctx, const void *d_grad, int row_type, uin
     const OnDevice guard(ctx->device);
     ROWS_CUDA(guard.status);
     auto s = static_cast<cudaStream_t>(stream);
-    const uint32_t most = most_of(row_type), v0 = count ? in.width(most) : most, v1 = out.width(most), v = v0 < v1 ? v0 : v1;
+    const uint32_t most = values_of(row_type), v = min_of(count ? in.width(most) : most, out.width(most));
     const GradScratch w(d_workspace, n, count, dim);
     const uint32_t items = (uint32_t) count, row_bytes = dim * bytes_of(grad_type);
     // Rows are cleared where the memory is idle: a share with each launch of the sort, whether an id names them or not, as long as ids are
     // few beside rows; the rest by the kernel that joins, which by then knows the rows that no id names.
     uint32_t clear_each = (128u << 10) / row_bytes, cleared = 0;   // a CTA clears up to 128 KB
     clear_each = clear_each < 1 ? 1 : clear_each > 256 ? 256 : clear_each;
-    GradArgs a{nullptr, items, (uint32_t) n, dim, dim / v, 32, 1, w.chunk, scale, grad_stride, table_grad_stride, accumulate, w.partial, table_grad_stride == dim ? row_bytes : 0, Div(row_bytes), 0, 0, clear_each};
-    if (count <= kFewIds) {
-        a.lanes = 256;
+    GradArgs a{nullptr, items, (uint32_t) n, dim, dim / v, 32, 1, w.chunk, scale, accumulate, w.partial, Div(row_bytes), 0, 0, clear_each};
+    // f(a value of the rows' type, one of the result's, the width)
+    auto with_types = [&](auto f) {
+        return with_rows(row_type, v, [&](auto t, auto wd) { return grad_type == GLIDE_ROW_F32 ? f(t, float{}, wd) : f(t, t, wd); });
+    };
+    auto lanes_up_to = [&](uint32_t most) {
+        a.lanes = most;
         while (a.lanes > 1 && a.lanes / 2 >= a.words) a.lanes /= 2;
+    };
+    if (count <= kFewIds) {
         const uint64_t grid = count + (accumulate ? 0 : ceil_div(n, clear_each));
         if (grid == 0) return GLIDE_OK;
-        auto run = [&](auto t, auto o, auto wd) {
+        lanes_up_to(256);
+        ROWS_CUDA(with_types([&](auto t, auto o, auto wd) {
             using T = decltype(t);
             using O = decltype(o);
-            constexpr int V = decltype(wd)::value;
-            return launch(grad_few_kernel<T, O, V>, grid, 256, 0, s, false, static_cast<const T *>(d_grad), static_cast<O *>(d_table_grad), d_ids, a);
-        };
-        ROWS_CUDA(with_rows(row_type, v, [&](auto t, auto wd) { return grad_type == GLIDE_ROW_F32 ? run(t, float{}, wd) : run(t, t, wd); }));
+            return launch(grad_few_kernel<T, O, decltype(wd)::value>, grid, 256, 0, s, false, in.as<const T>(), out.as<O>(), d_ids, a);
+        }));
         return GLIDE_OK;
     }
     const uint64_t share = accumulate || count >= n / 2 ? 0 : kClearShare / row_bytes;
@@ -1279,21 +1365,20 @@ int glide_lookup_rows_grad(glide_ctx *ctx, const void *d_grad, int row_type, uin
     }
     a.sorted = sorted;
     a.clear_from = cleared;
-    while (a.lanes > 1 && a.lanes / 2 >= a.words) a.lanes /= 2;
+    lanes_up_to(32);
     a.slabs = (uint32_t) ceil_div(a.words, a.lanes);
-    const uint64_t chunks = ceil_div(items, a.chunk), join = ceil_div(chunks * a.slabs * a.lanes, 256), units = chunks < 2 ? 0 : (chunks - 1) * a.slabs;
-    const uint64_t zero = accumulate ? 0 : ceil_div(n - cleared, clear_each);
+    const uint64_t zero = accumulate ? 0 : ceil_div(n - cleared, clear_each), chunks = ceil_div(items, a.chunk);
+    const uint64_t join = ceil_div(chunks * a.slabs * a.lanes, 256), units = (chunks - 1) * a.slabs;
     ROWS_REQUIRE(join <= 0xffffffu && units <= 0x7fffffffu && join + zero <= 0x7fffffffu, GLIDE_ERR_UNSUPPORTED, "lookup_rows_grad: too many values in one call");   // threads are counted in 32 bits
     a.join_blocks = (uint32_t) join;
-    auto run = [&](auto t, auto o, auto wd) {
+    ROWS_CUDA(with_types([&](auto t, auto o, auto wd) {
         using T = decltype(t);
         using O = decltype(o);
         constexpr int V = decltype(wd)::value;
-        const cudaError_t e = launch(grad_join_kernel<T, O, V>, join + zero, 256, 0, s, true, static_cast<const T *>(d_grad), static_cast<O *>(d_table_grad), a);
+        const cudaError_t e = launch(grad_join_kernel<T, O, V>, join + zero, 256, 0, s, true, in.as<const T>(), out.as<O>(), a);
         if (e != cudaSuccess || units == 0) return e;
-        return launch(grad_fix_kernel<O, V>, ceil_div(units, 8), 256, 0, s, true, static_cast<O *>(d_table_grad), a, (uint32_t) units);
-    };
-    ROWS_CUDA(with_rows(row_type, v, [&](auto t, auto wd) { return grad_type == GLIDE_ROW_F32 ? run(t, float{}, wd) : run(t, t, wd); }));
+        return launch(grad_fix_kernel<O, V>, ceil_div(units, 8), 256, 0, s, true, out.as<O>(), a, (uint32_t) units);
+    }));
     return GLIDE_OK;
 }
 
@@ -1331,21 +1416,17 @@ int glide_dispatch_rows(glide_ctx *ctx, const void *d_rows, int row_type, uint64
         ROWS_CUDA(cudaMemsetAsync(d_segment_start, 0, (partitions + 1) * 4ull, s));
         return GLIDE_OK;
     }
-    const uint32_t e = bytes_of(row_type), most = 16 / e, v0 = in.width(most), v1 = out.width(most), v = v0 < v1 ? v0 : v1, words = dim / v;
-    const uint8_t *from = static_cast<const uint8_t *>(d_rows);
-    uint8_t *to = static_cast<uint8_t *>(d_sorted);
-    auto with_bytes = [&](auto run) {
-        switch (v * e) {
-            case 16: return run(Width<16>{});
-            case 8: return run(Width<8>{});
-            case 4: return run(Width<4>{});
-            default: return run(Width<2>{});
-        }
+    const uint32_t most = values_of(row_type), v = min_of(in.width(most), out.width(most)), words = dim / v;
+    // rows are copied as bits: f(a value as wide as theirs, the width)
+    auto with_bits = [&](auto f) {
+        if (row_type == GLIDE_ROW_F32) return with_width<4>(v, [&](auto wd) { return f(uint32_t{}, wd); });
+        return with_width<8>(v, [&](auto wd) { return f(uint16_t{}, wd); });
     };
     if (pairs <= kFewPairs) {
-        ROWS_CUDA(with_bytes([&](auto b) {
-            return launch(dispatch_small_kernel<decltype(b)::value>, count + 1, 256, (partitions + 1) * 4, s, false, from, row_stride * e, (uint32_t) count, words, d_choice, choices, partitions,
-                          to, sorted_stride * e, d_position, d_map, d_segment_start);
+        ROWS_CUDA(with_bits([&](auto t, auto wd) {
+            using T = decltype(t);
+            return launch(dispatch_small_kernel<T, decltype(wd)::value>, count + 1, 256, (partitions + 1) * 4, s, false, in.as<const T>(), dim, (uint32_t) count, words, d_choice, choices, partitions,
+                          out.as<T>(), d_position, d_map, d_segment_start);
         }));
         return GLIDE_OK;
     }
@@ -1353,17 +1434,17 @@ int glide_dispatch_rows(glide_ctx *ctx, const void *d_rows, int row_type, uint64
     const Digit digit{partitions, 0, bits_for(partitions + 1)};
     const ToPlaces places{d_position, d_map, d_segment_start, Div(choices)};
     ROWS_CUDA(sort_pass(Keys{d_choice, nullptr}, (uint32_t) pairs, digit, partitions + 1, w.counts, w.totals, w.ranks, places, false, s, [] { return Clear{}; }));
-    const uint64_t each = 0x7fff0000u / words;   // rows of a launch: its words are counted in 31 bits
-    for (uint64_t r0 = 0; r0 < count; r0 += each) {
-        const uint32_t rows = (uint32_t) (count - r0 < each ? count - r0 : each), units = rows * words;
-        ROWS_CUDA(with_bytes([&](auto b) {
-            constexpr int B = decltype(b)::value;
-            const uint8_t *part = from + r0 * row_stride * e;
-            const uint32_t *position = d_position + r0 * choices;
-            if (units <= 256 * 1024) return launch(dispatch_kernel<B, 1>, ceil_div(units, 256), 256, 0, s, r0 == 0, part, row_stride * e, units, Div(words), choices, position, to, sorted_stride * e);
-            return launch(dispatch_kernel<B, 4>, ceil_div(units, 1024), 256, 0, s, r0 == 0, part, row_stride * e, units, Div(words), choices, position, to, sorted_stride * e);
-        }));
-    }
+    ROWS_CUDA(with_bits([&](auto t, auto wd) {
+        using T = decltype(t);
+        return in_parts(count, words, [&](uint64_t r0, uint32_t rows) {
+            const uint32_t units = rows * words;
+            auto go = [&](auto u) {
+                return launch(dispatch_kernel<T, decltype(wd)::value, decltype(u)::value>, ceil_div(units, 256 * decltype(u)::value), 256, 0, s, r0 == 0, in.from(r0).as<const T>(), dim, units,
+                              Div(words), choices, d_position + r0 * choices, out.as<T>());
+            };
+            return units <= 256 * 1024 ? go(Number<1>{}) : go(Number<4>{});
+        });
+    }));
     return GLIDE_OK;
 }
 
@@ -1383,22 +1464,23 @@ int glide_combine_rows(glide_ctx *ctx, const void *d_sorted, int row_type, uint6
     const OnDevice guard(ctx->device);
     ROWS_CUDA(guard.status);
     auto s = static_cast<cudaStream_t>(stream);
-    const uint32_t most = most_of(row_type), v0 = in.width(most), v1 = out.width(most), v = v0 < v1 ? v0 : v1, words = dim / v;
-    const uint64_t each = 0x7fff0000u / words;   // rows of a launch: its words are counted in 31 bits
-    for (uint64_t r0 = 0; r0 < count; r0 += each) {
-        const uint32_t rows = (uint32_t) (count - r0 < each ? count - r0 : each), units = rows * words, grid = (uint32_t) ceil_div(units, 256);
-        const uint32_t *position = d_position + r0 * choices;
-        const float *weights = d_weights_or_null ? d_weights_or_null + r0 * choices : nullptr;
-        ROWS_CUDA(with_rows(row_type, v, [&](auto t, auto wd) {
-            using T = decltype(t);
-            constexpr int V = decltype(wd)::value;
-            const T *from = static_cast<const T *>(d_sorted);
-            T *to = static_cast<T *>(d_out) + r0 * out_stride;
-            if (choices <= 2) combine_kernel<T, V, 2><<<grid, 256, 0, s>>>(from, sorted_stride, (uint32_t) sorted_rows, position, choices, weights, units, Div(words), to, out_stride);
-            else combine_kernel<T, V, 8><<<grid, 256, 0, s>>>(from, sorted_stride, (uint32_t) sorted_rows, position, choices, weights, units, Div(words), to, out_stride);
-            return cudaGetLastError();
-        }));
-    }
+    const uint32_t most = values_of(row_type), v = min_of(in.width(most), out.width(most));
+    ROWS_CUDA(with_rows_or_shifted(row_type, v, [&](auto t, auto wd, auto wh) {
+        using T = decltype(t);
+        constexpr int V = decltype(wd)::value;
+        constexpr bool kWhole = decltype(wh)::value != 0;
+        const uint32_t words = pieces<V, T>(kWhole, dim);
+        return in_parts(count, words, [&](uint64_t r0, uint32_t rows) {
+            const uint32_t units = rows * words;
+            auto go = [&](auto k) {
+                return launch(combine_kernel<T, V, kWhole, decltype(k)::value>, ceil_div(units, 256), 256, 0, s, false, in.as<const T>(), (uint32_t) sorted_rows, dim, d_position + r0 * choices, choices,
+                              d_weights_or_null ? d_weights_or_null + r0 * choices : nullptr, units, Div(words), out.from(r0).as<T>());
+            };
+            if (choices <= 2) return go(Number<2>{});
+            if constexpr (kWhole) if (choices >= 8) return go(Number<8>{});
+            return go(Number<4>{});
+        });
+    }));
     return GLIDE_OK;
 }
 
@@ -1426,19 +1508,16 @@ int glide_combine_rows_grad(glide_ctx *ctx, const void *d_grad, int row_type, ui
     const OnDevice guard(ctx->device);
     ROWS_CUDA(guard.status);
     auto s = static_cast<cudaStream_t>(stream);
-    const uint32_t most = most_of(row_type), v0 = grad.width(most), v1 = in.width(most), v2 = out.width(most);
-    const uint32_t v01 = v0 < v1 ? v0 : v1, v = v01 < v2 ? v01 : v2, words = dim / v;
+    const uint32_t most = values_of(row_type), v = min_of(grad.width(most), min_of(in.width(most), out.width(most))), words = dim / v;
     ROWS_CUDA(with_rows(row_type, v, [&](auto t, auto wd) {
         using T = decltype(t);
-        constexpr int V = decltype(wd)::value;
-        auto go = [&](auto kk, auto uu, auto gg) {
-            constexpr int K = decltype(kk)::value, U = decltype(uu)::value, G = decltype(gg)::value;
-            return launch(combine_grad_kernel<T, V, K, U, G>, ceil_div(count, 256 / G), 256, 0, s, false, static_cast<const T *>(d_grad), grad_stride, (uint32_t) count, words,
-                          static_cast<const T *>(d_sorted), sorted_stride, (uint32_t) sorted_rows, d_position, choices, d_weights_or_null, static_cast<T *>(d_grad_sorted),
-                          grad_sorted_stride, d_grad_weights_or_null);
+        auto go = [&](auto k, auto u, auto g) {
+            constexpr int K = decltype(k)::value, U = decltype(u)::value, G = decltype(g)::value;
+            return launch(combine_grad_kernel<T, decltype(wd)::value, K, U, G>, ceil_div(count, 256 / G), 256, 0, s, false, grad.as<const T>(), (uint32_t) count, dim, words, in.as<const T>(),
+                          (uint32_t) sorted_rows, d_position, choices, d_weights_or_null, out.as<T>(), d_grad_weights_or_null);
         };
-        if (count <= 148 * 8 && words > 64) return choices <= 4 ? go(Width<4>{}, Width<1>{}, Width<256>{}) : go(Width<8>{}, Width<1>{}, Width<256>{});
-        return choices <= 2 ? go(Width<2>{}, Width<2>{}, Width<32>{}) : choices < 8 ? go(Width<4>{}, Width<1>{}, Width<32>{}) : go(Width<8>{}, Width<1>{}, Width<32>{});
+        if (count <= 148 * 8 && words > 64) return choices <= 4 ? go(Number<4>{}, Number<1>{}, Number<256>{}) : go(Number<8>{}, Number<1>{}, Number<256>{});
+        return choices <= 2 ? go(Number<2>{}, Number<2>{}, Number<32>{}) : choices < 8 ? go(Number<4>{}, Number<1>{}, Number<32>{}) : go(Number<8>{}, Number<1>{}, Number<32>{});
     }));
     return GLIDE_OK;
 }
