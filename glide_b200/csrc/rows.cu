@@ -183,6 +183,10 @@ __device__ __forceinline__ void put(O *row, int32_t start, uint32_t dim, const f
     }
 }
 
+// How many pieces of `each` bytes a lane keeps in flight to have `bytes` of them: narrow ones have to be many (40,500 rows of 2,463 fp32
+// looked up one by one: 183 us with 4 in flight, XX with 16).
+__host__ __device__ constexpr int in_flight(int bytes, int each, int most) { return bytes / each < 1 ? 1 : bytes / each > most ? most : bytes / each; }
+
 // Quotient by a number that is the same for a whole launch, by a multiplication (Granlund and Montgomery, 1994): exact for
 // dividends below 2^31.
 struct Div {
@@ -222,6 +226,33 @@ __global__ void __launch_bounds__(256) lookup_kernel(Rows<const T> table, uint32
 #pragma unroll
         for (int i = 0; i < V; i++) f[i] *= id[u] < n ? scale : 0.0f;   // what was not fetched is 0
         put<V, kWhole>(to[u], at[u], dim, f);
+    }
+}
+
+// The same with a warp a row: what belongs to the row is worked out once, not for every piece. Taken for many long rows (kLongRow).
+template<typename T, typename O, int V, bool kWhole, int U>
+__global__ void __launch_bounds__(256) lookup_long_kernel(Rows<const T> table, uint32_t n, uint32_t dim, const uint32_t *__restrict__ ids, uint32_t count, uint32_t words,
+                                                          float scale, Rows<O> out) {
+    const uint32_t row = blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (row >= count) return;
+    const uint32_t id = ids[row];
+    const bool there = id < n;
+    const T *from = table.row(id);
+    O *to = out.row(row);
+    const float by = there ? scale : 0.0f;   // what is not fetched is 0
+    for (uint32_t c = threadIdx.x & 31u; c < words; c += 32 * U) {
+        Piece<T, V, kWhole> piece[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) piece[u] = fetch<V, kWhole>(table, from, piece_start<V, kWhole>(to, c + u * 32), dim, there && c + u * 32 < words);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (c + u * 32 >= words) break;
+            float f[V];
+            unpack<T, V>(piece[u].word(), f);
+#pragma unroll
+            for (int i = 0; i < V; i++) f[i] *= by;
+            put<V, kWhole>(to, piece_start<V, kWhole>(to, c + u * 32), dim, f);
+        }
     }
 }
 
@@ -670,7 +701,7 @@ __device__ __forceinline__ void clear_rows(const Rows<O> &out, const GradArgs &a
 // where the run goes on in another chunk, to the chunk's partial sums (first: it came from the chunk before).
 template<typename T, typename O, int V>
 __global__ void __launch_bounds__(256, 4) grad_join_kernel(Rows<const T> grad, Rows<O> out, GradArgs a) {
-    constexpr int U = 4;
+    constexpr int U = in_flight(64, V * (int) sizeof(T), 8);
     wait_for_previous();
     if (blockIdx.x >= a.join_blocks) {
         const uint64_t r0 = a.clear_from + (uint64_t) (blockIdx.x - a.join_blocks) * a.clear_rows;
@@ -809,7 +840,7 @@ __global__ void __launch_bounds__(256) grad_few_kernel(Rows<const T> grad, Rows<
 // Runs over several chunks, whose first chunk's unit (a chunk and a slab) adds their partial sums and writes the row. A warp owns a unit and
 // adds short runs by itself, in order; the CTA's warps share the runs with more partial sums than kLongRun, each takes consecutive ones,
 // and the warps' sums are added in order.
-constexpr uint32_t kLongRun = 32;
+constexpr uint32_t kLongRun = 16;
 template<typename O, int V>
 __global__ void __launch_bounds__(256) grad_fix_kernel(Rows<O> out, GradArgs a, uint32_t units) {
     __shared__ float part[8][32][V];
@@ -819,12 +850,20 @@ __global__ void __launch_bounds__(256) grad_fix_kernel(Rows<O> out, GradArgs a, 
     auto add = [&](uint32_t chunk, uint32_t word, uint32_t s0, uint32_t s1, float (&acc)[V]) {   // partial sums s0 .. s1 - 1 of the run that starts in chunk
 #pragma unroll
         for (int i = 0; i < V; i++) acc[i] = 0.0f;
-#pragma unroll 8
-        for (uint32_t s = s0; s < s1; s++) {
-            float f[V];
-            load<float, V>(a.partial + (2ull * (chunk + s) + (s == 0 ? 1 : 0)) * a.dim + word * V, f);
+        constexpr int U = in_flight(128, 4 * V, 8);
+        for (uint32_t s = s0; s < s1; s += U) {
+            float f[U][V];
 #pragma unroll
-            for (int i = 0; i < V; i++) acc[i] += f[i];
+            for (int u = 0; u < U; u++) {
+                const uint32_t i = min(s + u, s1 - 1);
+                load<float, V>(a.partial + (2ull * (chunk + i) + (i == 0 ? 1 : 0)) * a.dim + word * V, f[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                if (s + u >= s1) break;
+#pragma unroll
+                for (int i = 0; i < V; i++) acc[i] += f[u][i];
+            }
         }
     };
     const uint32_t unit = blockIdx.x * 8 + warp;
@@ -911,6 +950,31 @@ __global__ void __launch_bounds__(256) dispatch_kernel(Rows<const T> rows, uint3
     }
 }
 
+// The same with a warp a row, for many long rows.
+template<typename T, int V, int U>
+__global__ void __launch_bounds__(256) dispatch_long_kernel(Rows<const T> rows, uint32_t dim, uint32_t count, uint32_t words, uint32_t choices,
+                                                            const uint32_t *__restrict__ position, Rows<T> sorted) {
+    wait_for_previous();
+    const uint32_t row = blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (row >= count) return;
+    const T *from = rows.row(row);
+    position += (uint64_t) row * choices;
+    for (uint32_t c = threadIdx.x & 31u; c < words; c += 32 * U) {
+        Piece<T, V, true> piece[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) piece[u] = fetch<V, true>(rows, from, (int32_t) ((c + u * 32) * V), dim, c + u * 32 < words);
+#pragma unroll 2
+        for (uint32_t j = 0; j < choices; j++) {
+            const uint32_t p = position[j];
+            if (p == kNone) continue;
+            T *to = sorted.row(p) + c * V;
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                if (c + u * 32 < words) __stcg(reinterpret_cast<WordOf<T, V> *>(to + u * 32 * V), piece[u].a);
+        }
+    }
+}
+
 // Few pairs: everything in one launch. A CTA owns one row; a warp finds a pair's place by comparing it with all pairs, then the CTA
 // copies the row. One CTA more counts the partitions.
 template<typename T, int V>
@@ -988,6 +1052,56 @@ __global__ void __launch_bounds__(256) combine_kernel(Rows<const T> sorted, uint
         }
     }
     put<V, kWhole>(to, at, dim, acc);
+}
+
+// The same with a warp a row, for many long rows: U of its pieces and those of K of its places are in flight.
+template<typename T, int V, bool kWhole, int K, int U>
+__global__ void __launch_bounds__(256) combine_long_kernel(Rows<const T> sorted, uint32_t sorted_rows, uint32_t dim, const uint32_t *__restrict__ position,
+                                                           uint32_t choices, const float *__restrict__ weights, uint32_t count, uint32_t words, Rows<T> out) {
+    const uint32_t row = blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (row >= count) return;
+    T *to = out.row(row);
+    position += (uint64_t) row * choices;
+    uint32_t p[K];
+    float w[K];
+    auto places = [&](uint32_t j0) {
+#pragma unroll
+        for (int j = 0; j < K; j++) {
+            p[j] = j0 + j < choices ? position[j0 + j] : kNone;
+            w[j] = weights && j0 + j < choices ? weights[(uint64_t) row * choices + j0 + j] : 1.0f;
+        }
+    };
+    places(0);
+    for (uint32_t c = threadIdx.x & 31u; c < words; c += 32 * U) {
+        float acc[U][V];
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int i = 0; i < V; i++) acc[u][i] = 0.0f;
+        for (uint32_t j0 = 0; j0 < choices; j0 += K) {
+            if (choices > K) places(j0);
+            Piece<T, V, kWhole> y[U][K];
+#pragma unroll
+            for (int u = 0; u < U; u++)
+#pragma unroll
+                for (int j = 0; j < K; j++)
+                    y[u][j] = fetch<V, kWhole>(sorted, sorted.row(p[j]), piece_start<V, kWhole>(to, c + u * 32), dim, p[j] < sorted_rows && c + u * 32 < words);
+#pragma unroll
+            for (int j = 0; j < K; j++) {
+                if (p[j] >= sorted_rows) continue;
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    float f[V];
+                    unpack<T, V>(y[u][j].word(), f);
+#pragma unroll
+                    for (int i = 0; i < V; i++) acc[u][i] = fmaf(w[j], f[i], acc[u][i]);
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (c + u * 32 < words) put<V, kWhole>(to, piece_start<V, kWhole>(to, c + u * 32), dim, acc[u]);
+    }
 }
 
 // grad_sorted[position[t,j]] = weight[t,j] * grad[t] and grad_weights[t,j] = <grad[t], sorted[position[t,j]]>: G lanes own a row,
@@ -1178,11 +1292,18 @@ template<typename F> cudaError_t in_parts(uint64_t count, uint32_t words, F f) {
     return cudaSuccess;
 }
 
+// Whether a warp a row is taken, rather than a thread a piece: rows of two pieces a lane at least, enough of them for 16 warps an SM, and
+// pieces so narrow that the work around each of them tells.
+bool long_rows(uint64_t rows, uint32_t words, uint32_t piece_bytes) { return piece_bytes < 16 && words >= 64 && rows >= 148 * 16; }
+
 template<typename T, typename O, int V, bool kWhole>
 cudaError_t launch_lookup(const Matrix &table, const uint32_t *ids, float scale, const Matrix &out, cudaStream_t stream) {
     const uint32_t words = pieces<V, O>(kWhole, out.dim);
     return in_parts(out.rows, words, [&](uint64_t r0, uint32_t rows) {
         const uint32_t units = rows * words;
+        if (long_rows(rows, words, kWhole ? V * sizeof(T) : 8))   // shifted pieces have more work around them, too
+            return launch(lookup_long_kernel<T, O, V, kWhole, kWhole ? in_flight(64, V * (int) sizeof(T), 16) : 4>, ceil_div(rows, 8), 256, 0, stream, false, table.as<const T>(), (uint32_t) table.rows, out.dim, ids + r0, rows, words, scale,
+                          out.from(r0).as<O>());
         auto go = [&](auto u) {
             return launch(lookup_kernel<T, O, V, kWhole, decltype(u)::value>, ceil_div(units, 256 * decltype(u)::value), 256, 0, stream, false, table.as<const T>(), (uint32_t) table.rows,
                           out.dim, ids + r0, units, Div(words), scale, out.from(r0).as<O>());
@@ -1438,6 +1559,9 @@ int glide_dispatch_rows(glide_ctx *ctx, const void *d_rows, int row_type, uint64
         using T = decltype(t);
         return in_parts(count, words, [&](uint64_t r0, uint32_t rows) {
             const uint32_t units = rows * words;
+            if (long_rows(rows, words, decltype(wd)::value * sizeof t))
+                return launch(dispatch_long_kernel<T, decltype(wd)::value, in_flight(64, decltype(wd)::value * (int) sizeof(T), 16)>, ceil_div(rows, 8), 256, 0, s, r0 == 0, in.from(r0).as<const T>(), dim, rows, words, choices, d_position + r0 * choices,
+                              out.as<T>());
             auto go = [&](auto u) {
                 return launch(dispatch_kernel<T, decltype(wd)::value, decltype(u)::value>, ceil_div(units, 256 * decltype(u)::value), 256, 0, s, r0 == 0, in.from(r0).as<const T>(), dim, units,
                               Div(words), choices, d_position + r0 * choices, out.as<T>());
@@ -1473,7 +1597,12 @@ int glide_combine_rows(glide_ctx *ctx, const void *d_sorted, int row_type, uint6
         return in_parts(count, words, [&](uint64_t r0, uint32_t rows) {
             const uint32_t units = rows * words;
             auto go = [&](auto k) {
-                return launch(combine_kernel<T, V, kWhole, decltype(k)::value>, ceil_div(units, 256), 256, 0, s, false, in.as<const T>(), (uint32_t) sorted_rows, dim, d_position + r0 * choices, choices,
+                constexpr int K = decltype(k)::value, U = kWhole ? in_flight(128 / K, V * (int) sizeof(T), 8) : K == 2 ? 2 : 1;
+                // with a few choices, of which many may be missing, a thread a piece has too little in flight, whatever the width
+                if (long_rows(rows, words, kWhole && K != 4 ? V * sizeof t : kWhole ? 8 : 16))
+                    return launch(combine_long_kernel<T, V, kWhole, K, U>, ceil_div(rows, 8), 256, 0, s, false, in.as<const T>(), (uint32_t) sorted_rows, dim, d_position + r0 * choices, choices,
+                                  d_weights_or_null ? d_weights_or_null + r0 * choices : nullptr, rows, words, out.from(r0).as<T>());
+                return launch(combine_kernel<T, V, kWhole, K>, ceil_div(units, 256), 256, 0, s, false, in.as<const T>(), (uint32_t) sorted_rows, dim, d_position + r0 * choices, choices,
                               d_weights_or_null ? d_weights_or_null + r0 * choices : nullptr, units, Div(words), out.from(r0).as<T>());
             };
             if (choices <= 2) return go(Number<2>{});
@@ -1511,13 +1640,13 @@ int glide_combine_rows_grad(glide_ctx *ctx, const void *d_grad, int row_type, ui
     const uint32_t most = values_of(row_type), v = min_of(grad.width(most), min_of(in.width(most), out.width(most))), words = dim / v;
     ROWS_CUDA(with_rows(row_type, v, [&](auto t, auto wd) {
         using T = decltype(t);
-        auto go = [&](auto k, auto u, auto g) {
-            constexpr int K = decltype(k)::value, U = decltype(u)::value, G = decltype(g)::value;
-            return launch(combine_grad_kernel<T, decltype(wd)::value, K, U, G>, ceil_div(count, 256 / G), 256, 0, s, false, grad.as<const T>(), (uint32_t) count, dim, words, in.as<const T>(),
-                          (uint32_t) sorted_rows, d_position, choices, d_weights_or_null, out.as<T>(), d_grad_weights_or_null);
+        auto go = [&](auto k, auto g) {
+            constexpr int V = decltype(wd)::value, K = decltype(k)::value, G = decltype(g)::value, U = in_flight(64 / K, V * (int) sizeof(T), 8);
+            return launch(combine_grad_kernel<T, V, K, U, G>, ceil_div(count, 256 / G), 256, 0, s, false, grad.as<const T>(), (uint32_t) count, dim, words, in.as<const T>(), (uint32_t) sorted_rows,
+                          d_position, choices, d_weights_or_null, out.as<T>(), d_grad_weights_or_null);
         };
-        if (count <= 148 * 8 && words > 64) return choices <= 4 ? go(Number<4>{}, Number<1>{}, Number<256>{}) : go(Number<8>{}, Number<1>{}, Number<256>{});
-        return choices <= 2 ? go(Number<2>{}, Number<2>{}, Number<32>{}) : choices < 8 ? go(Number<4>{}, Number<1>{}, Number<32>{}) : go(Number<8>{}, Number<1>{}, Number<32>{});
+        if (count <= 148 * 8 && words > 64) return choices <= 4 ? go(Number<4>{}, Number<256>{}) : go(Number<8>{}, Number<256>{});
+        return choices <= 2 ? go(Number<2>{}, Number<32>{}) : choices < 8 ? go(Number<4>{}, Number<32>{}) : go(Number<8>{}, Number<32>{});
     }));
     return GLIDE_OK;
 }
