@@ -518,6 +518,13 @@ class GLIDE:
                                             int(self.metric), _ptr(h_ids), _ptr(h_dists)))
         return h_ids, h_dists
 
+    def lookup(self, d_ids: torch.Tensor, scale: float = 1.0, out: torch.Tensor | None = None) -> torch.Tensor:
+        """The rows of the index with these ids (an int32 tensor of uint32 patterns on the device, such as ``search`` and
+        ``bruteforce_knn`` of this module return), times `scale`: d_ids.shape + (dim,), zeros for 0xffffffff. Ordered on torch's
+        current stream, without a wait (``rows.lookup_rows``)."""
+        from . import rows
+        return rows.lookup_rows(self.ctx, self.d_data, d_ids, scale, out)
+
     def search_pipe(self, max_queries: int, max_top_k: int, depth: int = 3) -> "SearchPipe":
         """Host-buffer search with `depth` batches in flight (`glide_search_pipe_*`)."""
         return SearchPipe(self, max_queries, max_top_k, depth)

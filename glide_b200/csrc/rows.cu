@@ -31,7 +31,7 @@ constexpr uint32_t kFewPairs = 2048;        // pairs that dispatch_rows places a
 constexpr uint32_t kFewIds = 1024;          // ids whose gradient takes one launch
 constexpr uint32_t kMaxPassBits = 11;       // digits of a pass
 constexpr uint32_t kMaxFusedCounts = 16384; // counts (tiles x buckets) that every CTA of the second kernel adds up by itself
-constexpr uint32_t kClearShare = 24u << 20; // bytes of a gradient that are cleared beside each launch of its sort
+constexpr uint32_t kClearShare = 48u << 20; // bytes of a gradient that are cleared beside each launch of its sort
 
 // ---- rows as words ----------------------------------------------------------------------------------------
 // A kernel handles a row in pieces of V values, a word of up to 16 bytes of its input: as many as the addresses, strides and lengths of
@@ -866,10 +866,10 @@ __global__ void __launch_bounds__(256) grad_fix_kernel(Rows<O> out, GradArgs a, 
             }
         }
     };
-    const uint32_t unit = blockIdx.x * 8 + warp;
+    const uint32_t unit = blockIdx.x * 8 + warp, starts = units / a.slabs;   // chunk by chunk, so that the slabs of a long run fall to several CTAs
     uint32_t last = 0;   // the run's last chunk; 0: no run starts here and goes on
     if (unit < units) {
-        const uint32_t chunk = unit / a.slabs, word = (unit - chunk * a.slabs) * a.lanes + lane;
+        const uint32_t slab = unit / starts, chunk = unit - slab * starts, word = slab * a.lanes + lane;
         const uint64_t c0 = (uint64_t) chunk * a.chunk, c1 = c0 + a.chunk;   // below a.items, as the last chunk has no unit
         const uint32_t id = a.key(c1 - 1);
         if (id < a.n && a.key(c1) == id && !(a.key(c0) == id && c0 > 0 && a.key(c0 - 1) == id)) {
@@ -903,7 +903,7 @@ __global__ void __launch_bounds__(256) grad_fix_kernel(Rows<O> out, GradArgs a, 
     for (uint32_t f = 0; f < found; f += at_once) {
         const bool there = f + warp / each < found;
         const uint32_t u = units_of[there ? f + warp / each : 0];
-        const uint32_t chunk = (blockIdx.x * 8 + u) / a.slabs, word = (blockIdx.x * 8 + u - chunk * a.slabs) * a.lanes + lane;
+        const uint32_t slab = (blockIdx.x * 8 + u) / starts, chunk = blockIdx.x * 8 + u - slab * starts, word = slab * a.lanes + lane;
         const uint32_t sums = long_last[u] - chunk + 1, part_sums = (sums + each - 1) / each, s0 = min(share * part_sums, sums), s1 = min(s0 + part_sums, sums);
         const bool mine = there && lane < a.lanes && word < a.words;
         float acc[V];
@@ -1229,7 +1229,7 @@ struct Matrix {
     uint32_t dim;
     int type;
     uint64_t bytes() const { return rows == 0 ? 0 : ((rows - 1) * stride + dim) * bytes_of(type); }
-    bool sized() const { return stride <= (1ull << 40) && rows <= (1ull << 32); }
+    bool sized() const { return rows == 0 || stride <= (1ull << 60) / rows; }   // its bytes fit 64 bits
     // The most values (1, 2, 4 or 8) that a word may hold so that every word of every row is aligned, words of 16 bytes at most.
     uint32_t width(uint32_t most) const {
         const uint64_t e = bytes_of(type);
@@ -1346,10 +1346,10 @@ struct GradScratch {
         bits = bits_for(n + 1);             // ids 0 .. n - 1, and n for none
         passes = (bits + kMaxPassBits - 1) / kMaxPassBits;
         pass_bits = (bits + passes - 1) / passes;
-        // Long chunks leave few partial sums, short ones many groups of lanes to work: as long as some 32 warps an SM remain
+        // Long chunks leave few partial sums, short ones many groups of lanes to work: as long as some 16 warps an SM remain
         // (counted for words of 16 bytes of bf16), 8 to 128.
         chunk = 8;
-        while (chunk < 128 && count * dim / 256 / chunk >= 2 * 148 * 32) chunk *= 2;
+        while (chunk < 128 && count * dim / 256 / chunk >= 2 * 148 * 16) chunk *= 2;
         uint64_t at = 0;
         auto take = [&](uint64_t size) {
             const uint64_t here = at;
@@ -1399,7 +1399,7 @@ int glide_lookup_rows(glide_ctx *ctx, const void *d_table, int row_type, uint64_
     ROWS_REQUIRE(dim <= kMaxDim && count <= 0x7fffffffu, GLIDE_ERR_UNSUPPORTED, "lookup_rows: rows of more than 2^20 values or more than 2^31 - 1 ids");
     if (count == 0) return GLIDE_OK;
     ROWS_REQUIRE(d_table && d_ids && d_out, GLIDE_ERR_BAD_ARG, "lookup_rows: null pointer");
-    ROWS_REQUIRE(table.sized() && out.sized() && (out_stride >= dim || count == 1), GLIDE_ERR_BAD_ARG, "lookup_rows: rows of the result overlap, or a stride is beyond 2^40");
+    ROWS_REQUIRE(table.sized() && out.sized() && (out_stride >= dim || count == 1), GLIDE_ERR_BAD_ARG, "lookup_rows: rows of the result overlap, or it is beyond 2^60 values");
     ROWS_REQUIRE(aligned(table) && aligned(out) && reinterpret_cast<uintptr_t>(d_ids) % 4 == 0, GLIDE_ERR_BAD_ARG, "lookup_rows: a pointer is not aligned to its type");
     ROWS_REQUIRE(!overlap(out, table) && !overlap(d_out, out.bytes(), d_ids, count * 4), GLIDE_ERR_BAD_ARG, "lookup_rows: the result overlaps an input");
     const OnDevice guard(ctx->device);
@@ -1427,7 +1427,7 @@ int glide_lookup_rows_grad(glide_ctx *ctx, const void *d_grad, int row_type, uin
     ROWS_REQUIRE(dim >= 1 && n >= 1 && n <= kNone, GLIDE_ERR_BAD_ARG, "lookup_rows_grad: a table has 1 to 2^32 - 1 rows of at least one value");
     ROWS_REQUIRE(dim <= kMaxDim && count <= 0x7fffffffu, GLIDE_ERR_UNSUPPORTED, "lookup_rows_grad: rows of more than 2^20 values or more than 2^31 - 1 ids");
     ROWS_REQUIRE(d_table_grad && (count == 0 || (d_grad && d_ids)), GLIDE_ERR_BAD_ARG, "lookup_rows_grad: null pointer");
-    ROWS_REQUIRE(in.sized() && out.sized() && (table_grad_stride >= dim || n == 1), GLIDE_ERR_BAD_ARG, "lookup_rows_grad: rows of the result overlap, or a stride is beyond 2^40");
+    ROWS_REQUIRE(in.sized() && out.sized() && (table_grad_stride >= dim || n == 1), GLIDE_ERR_BAD_ARG, "lookup_rows_grad: rows of the result overlap, or it is beyond 2^60 values");
     ROWS_REQUIRE(aligned(in) && aligned(out) && reinterpret_cast<uintptr_t>(d_ids) % 4 == 0, GLIDE_ERR_BAD_ARG, "lookup_rows_grad: a pointer is not aligned to its type");
     const size_t need = glide_lookup_rows_grad_workspace(n, dim, count);
     ROWS_REQUIRE(workspace_bytes >= need && (need == 0 || d_workspace), GLIDE_ERR_BAD_ARG, "lookup_rows_grad: the workspace has %zu bytes, %zu are needed", workspace_bytes, need);
@@ -1518,7 +1518,7 @@ int glide_dispatch_rows(glide_ctx *ctx, const void *d_rows, int row_type, uint64
     const uint64_t pairs = count * choices;
     const Matrix in{d_rows, count, row_stride, dim, row_type}, out{d_sorted, pairs, sorted_stride, dim, row_type};
     ROWS_REQUIRE(d_segment_start && (count == 0 || (d_rows && d_choice && d_sorted && d_position && d_map)), GLIDE_ERR_BAD_ARG, "dispatch_rows: null pointer");
-    ROWS_REQUIRE(in.sized() && out.sized() && (sorted_stride >= dim || pairs <= 1), GLIDE_ERR_BAD_ARG, "dispatch_rows: rows of the result overlap, or a stride is beyond 2^40");
+    ROWS_REQUIRE(in.sized() && out.sized() && (sorted_stride >= dim || pairs <= 1), GLIDE_ERR_BAD_ARG, "dispatch_rows: rows of the result overlap, or it is beyond 2^60 values");
     ROWS_REQUIRE(aligned(in) && aligned(out) && (reinterpret_cast<uintptr_t>(d_choice) | reinterpret_cast<uintptr_t>(d_position) | reinterpret_cast<uintptr_t>(d_map) | reinterpret_cast<uintptr_t>(d_segment_start)) % 4 == 0, GLIDE_ERR_BAD_ARG, "dispatch_rows: a pointer is not aligned to its type");
     const size_t need = glide_dispatch_rows_workspace(count, choices, partitions);
     ROWS_REQUIRE(workspace_bytes >= need && (need == 0 || d_workspace), GLIDE_ERR_BAD_ARG, "dispatch_rows: the workspace has %zu bytes, %zu are needed", workspace_bytes, need);
@@ -1582,7 +1582,7 @@ int glide_combine_rows(glide_ctx *ctx, const void *d_sorted, int row_type, uint6
     if (count == 0) return GLIDE_OK;
     const Matrix in{d_sorted, sorted_rows, sorted_stride, dim, row_type}, out{d_out, count, out_stride, dim, row_type};
     ROWS_REQUIRE((d_sorted || sorted_rows == 0) && d_position && d_out, GLIDE_ERR_BAD_ARG, "combine_rows: null pointer");
-    ROWS_REQUIRE(in.sized() && out.sized() && (out_stride >= dim || count == 1), GLIDE_ERR_BAD_ARG, "combine_rows: rows of the result overlap, or a stride is beyond 2^40");
+    ROWS_REQUIRE(in.sized() && out.sized() && (out_stride >= dim || count == 1), GLIDE_ERR_BAD_ARG, "combine_rows: rows of the result overlap, or it is beyond 2^60 values");
     ROWS_REQUIRE(aligned(in) && aligned(out) && (reinterpret_cast<uintptr_t>(d_position) | reinterpret_cast<uintptr_t>(d_weights_or_null)) % 4 == 0, GLIDE_ERR_BAD_ARG, "combine_rows: a pointer is not aligned to its type");
     ROWS_REQUIRE(!overlap(out, in) && !overlap(d_out, out.bytes(), d_position, count * choices * 4) && !overlap(d_out, out.bytes(), d_weights_or_null, d_weights_or_null ? count * choices * 4 : 0), GLIDE_ERR_BAD_ARG, "combine_rows: the result overlaps an input");
     const OnDevice guard(ctx->device);
@@ -1625,7 +1625,7 @@ int glide_combine_rows_grad(glide_ctx *ctx, const void *d_grad, int row_type, ui
     const uint64_t pairs = count * choices;
     const Matrix grad{d_grad, count, grad_stride, dim, row_type}, in{d_sorted, sorted_rows, sorted_stride, dim, row_type}, out{d_grad_sorted, sorted_rows, grad_sorted_stride, dim, row_type};
     ROWS_REQUIRE(d_grad && d_position && (sorted_rows == 0 || (d_sorted && d_grad_sorted)), GLIDE_ERR_BAD_ARG, "combine_rows_grad: null pointer");
-    ROWS_REQUIRE(grad.sized() && in.sized() && out.sized() && (grad_sorted_stride >= dim || sorted_rows <= 1), GLIDE_ERR_BAD_ARG, "combine_rows_grad: rows of the result overlap, or a stride is beyond 2^40");
+    ROWS_REQUIRE(grad.sized() && in.sized() && out.sized() && (grad_sorted_stride >= dim || sorted_rows <= 1), GLIDE_ERR_BAD_ARG, "combine_rows_grad: rows of the result overlap, or it is beyond 2^60 values");
     ROWS_REQUIRE(aligned(grad) && aligned(in) && aligned(out) && (reinterpret_cast<uintptr_t>(d_position) | reinterpret_cast<uintptr_t>(d_weights_or_null) | reinterpret_cast<uintptr_t>(d_grad_weights_or_null)) % 4 == 0, GLIDE_ERR_BAD_ARG, "combine_rows_grad: a pointer is not aligned to its type");
     {
         struct Range { const void *p; uint64_t n; } r[] = {{d_grad, grad.bytes()}, {d_sorted, in.bytes()}, {d_position, pairs * 4}, {d_weights_or_null, d_weights_or_null ? pairs * 4 : 0},

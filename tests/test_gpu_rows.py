@@ -66,7 +66,8 @@ def _lookup_want(table, ids, scale):
 
 @pytest.mark.parametrize("dtype", TYPES + [torch.uint8])
 @pytest.mark.parametrize("n,dim,shape,scale", [(1, 1, (1,), 1.0), (7, 3, (5,), 2.5), (100, 100, (13, 10), 1.0), (1000, 128, (64, 10), 11.314),
-                                               (50, 33, (1000,), 1.0), (300, 960, (301,), 0.1), (17, 4096, (3, 3), 64.0), (40, 1030, (2000,), 1.0)])
+                                               (50, 33, (1000,), 1.0), (300, 960, (301,), 0.1), (17, 4096, (3, 3), 64.0), (40, 1030, (2000,), 1.0),
+                                               (700, 129, (3000,), 1.0), (300, 1001, (2400, 2), 1.5), (90, 520, (5000,), 1.0)])
 def test_lookup(gpu_ctx, dtype, n, dim, shape, scale):
     table = torch.randint(0, 256, (n, dim), generator=_gen(1), device="cuda", dtype=torch.uint8) if dtype == torch.uint8 else _randn((n, dim), dtype, 1)
     ids = _ids(shape, n, 2)
@@ -121,6 +122,23 @@ def test_lookup_offsets_pass_32_bits(gpu_ctx):
     untouched[ids.long()] = False
     for part in (slice(0, 1000), slice(1_048_000, 1_049_000), slice(n - 10_000, n)):     # each holds rows that ids name
         assert (table[part][untouched[part]] == 0).all()
+
+
+def test_more_pieces_than_a_launch_counts(gpu_ctx):
+    """2,200,000 rows of 1,001 fp32 values, one value a piece: more than 2^31 pieces, so the calls are made of two launches."""
+    count, dim = 2_200_000, 1_001
+    table = _randn((7, dim), torch.float32, 26)
+    ids = torch.randint(0, 7, (count,), generator=_gen(27), device="cuda", dtype=torch.int32)
+    out = rows.lookup_rows(gpu_ctx, table, ids)
+
+    def same(got, want_ids):
+        return all(torch.equal(got[a:a + 100_000], table[want_ids[a:a + 100_000].long()]) for a in range(0, count, 100_000))
+    assert same(out, ids)
+    d = rows.dispatch_rows(gpu_ctx, out, ids[:, None].contiguous(), 7)
+    assert same(d.d_sorted, torch.repeat_interleave(torch.arange(7, device="cuda"), torch.diff(d.d_segment_start).long()))
+    out.zero_()
+    rows.dispatch_rows_grad(gpu_ctx, d.d_sorted, d.d_position, out=out)
+    assert same(out, ids)
 
 
 # ---- gradient of a lookup ---------------------------------------------------------------------------------------
@@ -257,7 +275,7 @@ def _check_dispatch(got, data, choice, partitions):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("count,dim,choices,partitions", [(1, 1, 1, 1), (1, 64, 8, 64), (3, 100, 2, 5), (64, 256, 8, 256), (500, 33, 3, 7), (257, 520, 1, 1024), (2049, 12, 2, 4096),
-                                                          (1000, 8, 128, 130), (5000, 40, 2, 1), (9, 4096, 4, 3), (300, 130, 6, 2048), (20_001, 6, 2, 300)])
+                                                          (1000, 8, 128, 130), (5000, 40, 2, 1), (9, 4096, 4, 3), (300, 130, 6, 2048), (20_001, 6, 2, 300), (2500, 129, 3, 40), (2400, 1001, 2, 5), (3000, 2048, 2, 64)])
 def test_dispatch(gpu_ctx, dtype, count, dim, choices, partitions):
     data, choice = _randn((count, dim), dtype, 30), _choice(count, choices, partitions, 31)
     keep = _randn((count * choices, dim), dtype, 32)
@@ -325,7 +343,8 @@ def _combine_case(dtype, count, dim, choices, empty, seed):
     return _randn((count * choices, dim), dtype, seed + 1), position, torch.rand((count, choices), generator=_gen(seed + 2), device="cuda") * 2 - 1
 
 
-COMBINE = [(1, 1, 1, 0.0), (1, 64, 8, 0.0), (64, 2048, 8, 0.1), (301, 100, 2, 0.2), (77, 33, 3, 0.1), (19, 1030, 9, 0.1), (40, 12, 128, 0.5), (1000, 520, 1, 0.1), (5000, 24, 4, 0.1), (33, 130, 17, 0.0)]
+COMBINE = [(1, 1, 1, 0.0), (1, 64, 8, 0.0), (64, 2048, 8, 0.1), (301, 100, 2, 0.2), (77, 33, 3, 0.1), (19, 1030, 9, 0.1), (40, 12, 128, 0.5), (1000, 520, 1, 0.1), (5000, 24, 4, 0.1), (33, 130, 17, 0.0), (2500, 129, 3, 0.3),
+           (2400, 1001, 2, 0.1), (2400, 1001, 5, 0.1), (2500, 520, 6, 0.6), (2400, 258, 9, 0.1), (1100, 600, 9, 0.1)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -458,6 +477,8 @@ def test_a_search_a_lookup_and_the_gradient_of_the_rows_found(gpu_ctx):
     ids, _ = api.bruteforce_knn(ctx, table, queries, 10)
     found = rows.lookup_rows(ctx, table, ids)
     assert torch.equal(found, table[ids.long()])
+    index = api.GLIDE(ctx, 16, table, table[:4])
+    assert torch.equal(index.lookup(ids), found) and torch.equal(index.lookup(ids, 2.0), found * 2)
     grad = torch.randint(-9, 10, found.shape, generator=_gen(85), device="cuda").float()
     got = rows.lookup_rows_grad(ctx, grad, ids, 3000)
     want = torch.zeros((3000, 48), device="cuda").index_add_(0, ids.long().reshape(-1), grad.reshape(-1, 48))
