@@ -3,9 +3,10 @@
 // rows) or an assignment (partitions to rows) and precede an index (the table it is built over); the reference has
 // no counterpart. All calls enqueue on the caller's stream and return; scratch is the caller's.
 //
-// Everything here is bound by bytes. Rows are read and written in the widest words their addresses allow (16 bytes where
-// base, stride and length are multiples of it), sums are fp32 in an order that the arguments alone determine, and each
-// value is rounded once, when it is stored.
+// Everything here is bound by bytes, or by launches where rows are few. Rows are read and written in the widest words their
+// addresses allow (16 bytes where base, stride and length are multiples of it), sums are fp32 in an order that the arguments
+// alone determine, and each value is rounded once, when it is stored. Times in the comments are of one call in a captured graph on
+// inputs larger than L2, shares are of the measured copy rate (6.55 TB/s).
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
@@ -26,20 +27,20 @@ constexpr uint32_t kMaxChoices = 128;       // as many as glide_bruteforce_knn r
 constexpr uint32_t kMaxDim = 1u << 20;
 constexpr uint32_t kRounds = 8;             // items of a thread in the counting sort
 constexpr uint32_t kTileThreads = 256, kTile = kTileThreads * kRounds;
-constexpr uint32_t kFew = 4096;             // items that are sorted by comparing each with all
-constexpr uint32_t kFewPairs = 2048;        // pairs that dispatch_rows places and copies in one launch (2,000: 6 to 8 us, by tiles 8)
-constexpr uint32_t kFewIds = 1024;          // ids whose gradient takes one launch
-constexpr uint32_t kMaxPassBits = 11;       // digits of a pass
-constexpr uint32_t kMaxFusedCounts = 16384; // counts (tiles x buckets) that every CTA of the second kernel adds up by itself
-constexpr uint32_t kClearShare = 48u << 20; // bytes of a gradient that are cleared beside each launch of its sort
+constexpr uint32_t kFew = 4096;             // items that are sorted by comparing each with all (the gradient of 4,000 ids of 64 bf16: 15 us, of 4,097 in tiles: 20)
+constexpr uint32_t kFewPairs = 2048;        // pairs that dispatch_rows places and copies in one launch (2,000: 6 to 8 us, in tiles 8; 4,000: 14 to 19, in tiles 8 to 10)
+constexpr uint32_t kFewIds = 1024;          // ids whose gradient takes one launch (see grad_few_kernel)
+constexpr uint32_t kMaxPassBits = 11;       // bits of a pass's digit, at most
+constexpr uint32_t kMaxFusedCounts = 16384; // counts (tiles x buckets) that every CTA of the second kernel adds up by itself (64 x 1,001 of them: 19.5 us, scanned by a launch of their own 13.9)
+constexpr uint32_t kClearShare = 48u << 20; // bytes of a gradient that are cleared beside each launch of its sort (12 to 64 MB differ by 3 %)
 
 // ---- rows as words ----------------------------------------------------------------------------------------
 // A kernel handles a row in pieces of V values, a word of up to 16 bytes of its input: as many as the addresses, strides and lengths of
 // all matrices are multiples of. Rows of an odd number of 16-bit values (or of bytes) would leave an access for each value. Where that
 // costs most (lookup_kernel, combine_kernel) they have a second form, kWhole = false: a piece is what falls into a word of the row
 // that is WRITTEN, so that full words are stored, and what is read lies in two words beside each other, which are shifted into one;
-// words that would reach beyond the matrix are read value by value. 1,001 bf16 a row, both ways: 40,000 rows looked up 55 and 42 us,
-// 20,000 x 4 combined 119 and 62; but dispatched 71 and 94, the gradient of combine 115 and 170: there the shifting costs more.
+// words that would reach beyond the matrix are read value by value. 1,001 bf16 a row, value by value and shifted: 40,000 rows looked up
+// 46 and 38 us, 20,000 x 4 combined 88 and 65; but dispatched 56 and 94, the gradient of combine 94 and 170: the shifting costs more.
 template<int B> struct Word;
 template<> struct Word<16> { using type = uint4; };
 template<> struct Word<8> { using type = uint2; };
@@ -184,7 +185,7 @@ __device__ __forceinline__ void put(O *row, int32_t start, uint32_t dim, const f
 }
 
 // How many pieces of `each` bytes a lane keeps in flight to have `bytes` of them: narrow ones have to be many (40,500 rows of 2,463 fp32
-// looked up one by one: 183 us with 4 in flight, XX with 16).
+// looked up one by one: 183 us with 4 in flight, 119 with 16).
 __host__ __device__ constexpr int in_flight(int bytes, int each, int most) { return bytes / each < 1 ? 1 : bytes / each > most ? most : bytes / each; }
 
 // Quotient by a number that is the same for a whole launch, by a multiplication (Granlund and Montgomery, 1994): exact for
@@ -200,7 +201,9 @@ struct Div {
 
 // ---- lookup -------------------------------------------------------------------------------------------------
 // out[t] = scale * table[ids[t]], zeros for ids beyond the table (0xffffffff among them). A thread owns U pieces of the output, a
-// CTA's width apart, so that U loads are in flight once the ids (which a CTA shares through L1) have come.
+// CTA's width apart, so that U loads are in flight once the ids (which a CTA shares through L1) have come: 2 for large calls (1 takes a
+// quarter longer, 4 as long), 1 where 2 would leave SMs idle. 32,768 ids over 131,072 rows of 8 KB: 64 us, 88 % of the copy rate; bound by
+// DRAM and, a little, by the wait for the ids.
 template<typename T, typename O, int V, bool kWhole, int U>
 __global__ void __launch_bounds__(256) lookup_kernel(Rows<const T> table, uint32_t n, uint32_t dim, const uint32_t *__restrict__ ids, uint32_t units, Div words,
                                                      float scale, Rows<O> out) {
@@ -229,7 +232,7 @@ __global__ void __launch_bounds__(256) lookup_kernel(Rows<const T> table, uint32
     }
 }
 
-// The same with a warp a row: what belongs to the row is worked out once, not for every piece. Taken for many long rows (kLongRow).
+// The same with a warp a row: what belongs to the row is worked out once, not for every piece. Taken for many long rows of narrow pieces (long_rows).
 template<typename T, typename O, int V, bool kWhole, int U>
 __global__ void __launch_bounds__(256) lookup_long_kernel(Rows<const T> table, uint32_t n, uint32_t dim, const uint32_t *__restrict__ ids, uint32_t count, uint32_t words,
                                                           float scale, Rows<O> out) {
@@ -290,8 +293,9 @@ cudaError_t launch(void (*kernel)(P...), uint64_t grid, uint32_t block, uint32_t
 // its digit is the warp's running count plus the equal digits at lower lanes, and a scan over the warps' counts makes it the
 // rank in the tile. No atomics: the order depends on nothing but the keys. Few launches count most here (the data are 6 to 10
 // bytes an item): up to kFew items are sorted by one launch that compares each with all, more by two launches a pass while every CTA
-// of the second can add up the counts of all tiles, else by three. Tiles are small because their items' scattered stores leave an SM at
-// one sector a cycle: with 8,192 items to a tile a pass over 100,000 ids took 31 us.
+// of the second can add up the counts of all tiles, else by three. A launch takes 2 to 4 us of latency, whatever its size. Tiles are
+// small because their items' scattered stores leave an SM at one sector a cycle: in tiles of 8,192 a pass over 100,000 ids took 31 us,
+// in tiles of 2,048 it takes 10.
 struct Digit {
     uint32_t limit, shift, bits;   // keys beyond limit count as limit; bits: of the digit
     __device__ __forceinline__ uint32_t of(uint32_t key) const { return (min(key, limit) >> shift) & ((1u << bits) - 1); }
@@ -342,7 +346,7 @@ __device__ __forceinline__ uint32_t tile_item(uint32_t r) {   // of this thread,
 }
 
 // Ranks in the tile of this thread's items by their digits (kNone: no item), and the tile's count of each bucket through `put`.
-// Lanes of the same digit are found by a ballot for each bit (a match instruction took twice as long).
+// Lanes of the same digit are found by a ballot for each bit of it.
 template<typename Put>
 __device__ __forceinline__ void rank_tile(const uint32_t (&d)[kRounds], uint32_t bits, uint32_t buckets, uint16_t *warp_counts, uint32_t (&rank)[kRounds], Put put) {
     const uint32_t warps = blockDim.x >> 5, lane = threadIdx.x & 31u;
@@ -560,7 +564,7 @@ __global__ void __launch_bounds__(kTileThreads) bucket_place_kernel(Keys keys, u
 }
 
 // Few items: an item's place is the number of smaller keys and of equal ones before it. A CTA holds all keys in shared memory, `few_keys`
-// fills them; a warp counts for one item. 4,096 items take 6 us, two passes over tiles of them 14.
+// fills them; a warp counts for one item.
 __device__ __forceinline__ void few_keys(const uint32_t *__restrict__ keys, uint32_t items, uint32_t limit, uint4 *all) {
     uint32_t *to = reinterpret_cast<uint32_t *>(all);
 #pragma unroll 8
@@ -698,7 +702,10 @@ __device__ __forceinline__ void clear_rows(const Rows<O> &out, const GradArgs &a
 }
 
 // A group of lanes joins a chunk of sorted items over a slab of the row: the sum of a run of equal ids goes to the id's row, or,
-// where the run goes on in another chunk, to the chunk's partial sums (first: it came from the chunk before).
+// where the run goes on in another chunk, to the chunk's partial sums (first: it came from the chunk before). Consecutive items of a
+// sorted list make equal shares of any distribution of ids, be it one id. The other CTAs clear the rows that no id names.
+// 32,768 tokens over 131,072 rows of 8 KB (1.3 GB with the cleared rows): 222 us with its sort, 93 % of the copy rate; 100,000 ids over a
+// million rows of 512 bytes: 106 us, 81 %, of which the sort's latency is the rest.
 template<typename T, typename O, int V>
 __global__ void __launch_bounds__(256, 4) grad_join_kernel(Rows<const T> grad, Rows<O> out, GradArgs a) {
     constexpr int U = in_flight(64, V * (int) sizeof(T), 8);
@@ -924,7 +931,9 @@ __global__ void __launch_bounds__(256) grad_fix_kernel(Rows<O> out, GradArgs a, 
 }
 
 // ---- dispatch ---------------------------------------------------------------------------------------------------
-// Each row, read once, is copied to the places of its pairs. A thread has U words of rows in flight.
+// Each row, read once, is copied to the places of its pairs. A thread has U words of rows in flight. 16,384 x 8 rows of 4 KB: 93 us
+// of 104 with the sort, bound by the writes (5.6 TB/s). The other way round, sorted rows fetched by the map and written one behind the
+// other, takes 138: each row is read eight times.
 template<typename T, int V, int U>
 __global__ void __launch_bounds__(256) dispatch_kernel(Rows<const T> rows, uint32_t dim, uint32_t units, Div words, uint32_t choices,
                                                        const uint32_t *__restrict__ position, Rows<T> sorted) {
@@ -1018,7 +1027,8 @@ __global__ void __launch_bounds__(256) dispatch_small_kernel(Rows<const T> rows,
 }
 
 // ---- combine ----------------------------------------------------------------------------------------------------
-// out[t] = sum over j, ascending, of weight[t,j] * sorted[position[t,j]]; K pairs' pieces are in flight for each piece of a row.
+// out[t] = sum over j, ascending, of weight[t,j] * sorted[position[t,j]]; K pairs' pieces are in flight for each piece of a row: as many
+// as there are choices, up to 8. 16,384 x 8 rows of 4 KB: 92 us, 98 % of the copy rate.
 template<typename T, int V, bool kWhole, int K>
 __global__ void __launch_bounds__(256) combine_kernel(Rows<const T> sorted, uint32_t sorted_rows, uint32_t dim, const uint32_t *__restrict__ position,
                                                       uint32_t choices, const float *__restrict__ weights, uint32_t units, Div words, Rows<T> out) {
@@ -1106,7 +1116,8 @@ __global__ void __launch_bounds__(256) combine_long_kernel(Rows<const T> sorted,
 
 // grad_sorted[position[t,j]] = weight[t,j] * grad[t] and grad_weights[t,j] = <grad[t], sorted[position[t,j]]>: G lanes own a row,
 // and have U of its pieces and those of K of its places in flight. A warp a row beats a CTA a row (16,384 x 8 rows of 4 KB: 180 against
-// 205 us; 39,047 x 4 of 5 KB: 278 against 340) but where rows are few (64 x 8: 9.1 against 3.3; 1,000 x 4 of 8 KB: 22 against 16).
+// 205 us, 95 % of the copy rate; 39,047 x 4 of 5 KB: 278 against 340) but where rows are few (64 x 8: 9.1 against 3.3; 1,000 x 4 of 8 KB:
+// 22 against 16). grad is read once for K places.
 template<typename T, int V, int K, int U, int G>
 __global__ void __launch_bounds__(256) combine_grad_kernel(Rows<const T> grad, uint32_t count, uint32_t dim, uint32_t words, Rows<const T> sorted, uint32_t sorted_rows,
                                                            const uint32_t *__restrict__ position, uint32_t choices, const float *__restrict__ weights,
@@ -1309,7 +1320,7 @@ cudaError_t launch_lookup(const Matrix &table, const uint32_t *ids, float scale,
             return launch(lookup_kernel<T, O, V, kWhole, decltype(u)::value>, ceil_div(units, 256 * decltype(u)::value), 256, 0, stream, false, table.as<const T>(), (uint32_t) table.rows,
                           out.dim, ids + r0, units, Div(words), scale, out.from(r0).as<O>());
         };
-        return units <= 256 * 1024 ? go(Number<1>{}) : go(Number<4>{});
+        return units <= 256 * 1024 ? go(Number<1>{}) : go(Number<2>{});
     });
 }
 
@@ -1567,7 +1578,7 @@ int glide_dispatch_rows(glide_ctx *ctx, const void *d_rows, int row_type, uint64
                 return launch(dispatch_kernel<T, decltype(wd)::value, decltype(u)::value>, ceil_div(units, 256 * decltype(u)::value), 256, 0, s, r0 == 0, in.from(r0).as<const T>(), dim, units,
                               Div(words), choices, d_position + r0 * choices, out.as<T>());
             };
-            return units <= 256 * 1024 ? go(Number<1>{}) : go(Number<4>{});
+            return units <= 256 * 1024 ? go(Number<1>{}) : go(Number<2>{});
         });
     }));
     return GLIDE_OK;

@@ -39,7 +39,8 @@ def _on_device(ctx: Context, name: str, t: torch.Tensor):
 
 def _matrix(ctx: Context, name: str, t: torch.Tensor, types=_FLOATS) -> tuple[int, int, int]:
     """Address, type and stride between rows (in values) of a 2-D tensor."""
-    _on_device(ctx, name, t)
+    if not isinstance(t, torch.Tensor) or t.device != ctx.torch_device:
+        _on_device(ctx, name, t)
     kind = types.get(t.dtype)
     if kind is None:
         raise TypeError(f"{name} must be one of {', '.join(str(x) for x in types)}, got {t.dtype}")
@@ -53,7 +54,8 @@ def _matrix(ctx: Context, name: str, t: torch.Tensor, types=_FLOATS) -> tuple[in
 
 def _whole(ctx: Context, name: str, t: torch.Tensor, dtype: torch.dtype, shape=None) -> int:
     """The address of a contiguous tensor of 4-byte values."""
-    _on_device(ctx, name, t)
+    if not isinstance(t, torch.Tensor) or t.device != ctx.torch_device:
+        _on_device(ctx, name, t)
     if t.dtype != dtype and not (dtype == torch.int32 and t.dtype == torch.uint32):
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
     if shape is not None and t.shape != shape:
@@ -89,9 +91,9 @@ def lookup_rows(ctx: Context, d_table: torch.Tensor, d_ids: torch.Tensor, scale:
     table, kind, stride = _matrix(ctx, "d_table", d_table, _TYPES)
     n, dim = d_table.shape
     ids = _whole(ctx, "d_ids", d_ids, torch.int32)
-    shape, dtype = (*d_ids.shape, dim), torch.float32 if kind == 1 else d_table.dtype
+    shape, dtype = d_ids.shape + (dim,), torch.float32 if kind == 1 else d_table.dtype
     if out is None:
-        out = d_table.new_empty(shape, dtype=dtype)
+        out = d_table.new_empty(shape, dtype=dtype) if kind == 1 else d_table.new_empty(shape)
         to, to_stride = out.data_ptr(), dim
     else:
         _check_result(ctx, out, shape, dtype)
@@ -142,9 +144,10 @@ def dispatch_rows(ctx: Context, d_rows: torch.Tensor, d_choice: torch.Tensor, pa
     else:
         _check_result(ctx, out, (pairs, dim), d_rows.dtype)
     to, _, to_stride = _matrix(ctx, "out", out)
-    d_map = d_choice.new_empty(pairs, dtype=torch.int32)
-    d_position = d_choice.new_empty((count, choices), dtype=torch.int32)
-    d_start = d_choice.new_empty(partitions + 1, dtype=torch.int32)
+    # results of ids have the type that the choices have: int32, or uint32 like them
+    d_map = d_choice.new_empty(pairs)
+    d_position = d_choice.new_empty((count, choices))
+    d_start = d_choice.new_empty(partitions + 1)
     need = ctx.lib.glide_dispatch_rows_workspace(count, choices, partitions)
     scratch = d_choice.new_empty(need, dtype=torch.uint8) if need else None
     ctx.check(ctx.lib.glide_dispatch_rows(ctx.handle, rows, kind, count, dim, stride, choice, choices, partitions, to, to_stride,
