@@ -23,7 +23,7 @@ _TYPES = {**_FLOATS, torch.uint8: 1}
 class Dispatched(NamedTuple):
     """What ``dispatch_rows`` returns. d_sorted [rows * choices, dim]: the rows by partition; d_map [rows * choices]: the row at each
     place, -1 behind the last; d_position [rows, choices]: the place of each choice, -1 for none; d_segment_start
-    [partitions + 1]: the first place of each partition, then the number of places taken."""
+    [partitions + 1]: the first place of each partition, then the number of places taken. Ids have the type of d_choice."""
     d_sorted: torch.Tensor
     d_map: torch.Tensor
     d_position: torch.Tensor
