@@ -232,6 +232,35 @@ def test_lookup_grad_of_a_broadcast_gradient_and_strided_results(gpu_ctx):
     assert torch.equal(whole[~mask], before[~mask])
 
 
+@pytest.mark.parametrize("dtype,out_type", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16), (torch.float16, torch.float32)])
+@pytest.mark.parametrize("count", [40, 1500, 6000, 30_000])
+@pytest.mark.parametrize("dim,stride,offset", [(100, 108, 0), (100, 100, 3), (20, 33, 1), (1, 1, 0), (1, 3, 1), (5, 5, 1), (7, 8, 0), (136, 136, 1), (264, 271, 0)])
+def test_lookup_grad_clears_what_no_id_names_and_nothing_else(gpu_ctx, dtype, out_type, count, dim, stride, offset):
+    """Results of every alignment, with many more rows than ids (cleared beside the sort) and with few (cleared by the join)."""
+    for n in (700, 20_011):
+        out, whole = _strided((n, dim), out_type, 28, stride, offset)
+        whole.fill_(float("nan"))
+        ids = _ids((count,), n, 29)
+        grad = torch.randint(-3, 4, (count, dim), generator=_gen(30), device="cuda").to(dtype)
+        rows.lookup_rows_grad(gpu_ctx, grad, ids, n, out=out)
+        there = ids >= 0
+        want = torch.zeros((n, dim), dtype=torch.float64, device="cuda").index_add_(0, ids[there].long(), grad[there].double())
+        assert torch.equal(out, want.to(out_type))        # whole numbers: exact sums, rounded once
+        mask = torch.zeros_like(whole, dtype=torch.bool)
+        mask.as_strided((n, dim), (stride, 1), offset).fill_(True)
+        assert whole[~mask].isnan().all()
+
+
+def test_ids_of_unsigned_type(gpu_ctx):
+    table = _randn((50, 24), torch.float32, 31)
+    ids = _ids((30,), 50, 32)
+    assert torch.equal(rows.lookup_rows(gpu_ctx, table, ids.view(torch.uint32)), rows.lookup_rows(gpu_ctx, table, ids))
+    data, choice = _randn((9, 24), torch.float32, 33), _ids((9, 2), 4, 34)
+    a, b = rows.dispatch_rows(gpu_ctx, data, choice, 4), rows.dispatch_rows(gpu_ctx, data, choice.view(torch.uint32), 4)
+    assert b.d_map.dtype == torch.uint32 and torch.equal(a.d_position, b.d_position.view(torch.int32))
+    assert torch.equal(rows.dispatch_rows_grad(gpu_ctx, b.d_sorted, b.d_position), rows.dispatch_rows_grad(gpu_ctx, a.d_sorted, a.d_position))
+
+
 def test_lookup_grad_is_the_derivative_of_lookup(gpu_ctx):
     """A linear map: <lookup(X), G> = <X, grad(G)> for any X and G. The products are of values of fp32, the sums in 64 bits; each side's
     fp32 rounding is bounded as above, by (terms + 3) u of the magnitudes."""
@@ -507,11 +536,12 @@ def test_calls_run_on_the_current_stream(gpu_ctx):
         _close(grad, want, _grad_tol(want, size, terms, torch.float32))
 
 
-def test_calls_are_captured_and_replayed(gpu_ctx):
+@pytest.mark.parametrize("shape", [1, 3, 10])       # one launch, few ids, tiles
+def test_calls_are_captured_and_replayed(gpu_ctx, shape):
     """One graph of all operators, replayed on new inputs in the same tensors, gives the bits of the calls themselves; a second graph, captured
     while the first lives, does not disturb it."""
     ctx, parts = gpu_ctx, 40
-    table, ids = _randn((5000, 96), torch.bfloat16, 100), _ids((700, 3), 5000, 101)
+    table, ids = _randn((5000, 96), torch.bfloat16, 100), _ids((700, shape), 5000, 101)
     data, choice = _randn((1500, 96), torch.bfloat16, 102), _choice(1500, 4, parts, 103)
     weights = torch.rand((1500, 4), generator=_gen(104), device="cuda")
     keep, keep2 = torch.zeros((6000, 96), dtype=torch.bfloat16, device="cuda"), torch.zeros((6000, 96), dtype=torch.bfloat16, device="cuda")
@@ -534,7 +564,7 @@ def test_calls_are_captured_and_replayed(gpu_ctx):
         graphs.append(g)
     for seed in (110, 120):
         table.copy_(_randn(table.shape, torch.bfloat16, seed))
-        ids.copy_(_ids((700, 3), 5000, seed + 1))
+        ids.copy_(_ids((700, shape), 5000, seed + 1))
         data.copy_(_randn(data.shape, torch.bfloat16, seed + 2))
         choice.copy_(_choice(1500, 4, parts, seed + 3, 0.4))
         for g, r in zip(graphs, results):
@@ -548,6 +578,35 @@ def test_calls_are_captured_and_replayed(gpu_ctx):
             for x, y in zip(replayed, work()):
                 assert torch.equal(x, y)
     del graphs, results
+
+
+def test_two_threads_with_a_context_each(gpu_ctx):
+    import threading
+    table = _randn((30_000, 64), torch.float32, 130)
+    work = []
+    for i in range(2):
+        ids, data, choice = _ids((9000 + i,), 30_000, 131 + i), _randn((5000, 40), torch.float32, 133 + i), _choice(5000, 2, 300, 135 + i)
+        work.append((api.Context(0), torch.cuda.Stream(), ids, data, choice))
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def run(i):
+        ctx, stream, ids, data, choice = work[i]
+        with torch.cuda.stream(stream):
+            for _ in range(10):
+                d = rows.dispatch_rows(ctx, data, choice, 300)
+                got[i] = [rows.lookup_rows_grad(ctx, rows.lookup_rows(ctx, table, ids), ids, 30_000), rows.dispatch_rows_grad(ctx, d.d_sorted, d.d_position), *d[1:]]
+        stream.synchronize()
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    for i in range(2):
+        _, _, ids, data, choice = work[i]
+        d = rows.dispatch_rows(gpu_ctx, data, choice, 300)
+        want = [rows.lookup_rows_grad(gpu_ctx, rows.lookup_rows(gpu_ctx, table, ids), ids, 30_000), rows.dispatch_rows_grad(gpu_ctx, d.d_sorted, d.d_position), *d[1:]]
+        assert all(torch.equal(x, y) for x, y in zip(got[i], want))
+        work[i][0].close()
 
 
 def test_the_current_device_stays(gpu_ctx):
