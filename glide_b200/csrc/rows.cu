@@ -345,13 +345,12 @@ __device__ __forceinline__ uint32_t tile_item(uint32_t r) {   // of this thread,
     return (threadIdx.x >> 5) * (kRounds * 32) + r * 32 + (threadIdx.x & 31u);
 }
 
-// Ranks in the tile of this thread's items by their digits (kNone: no item), and the tile's count of each bucket through `put`.
+// Ranks in the tile of this thread's items by their digits (kNone: no item), and the tile's count of each bucket through `put`;
+// warp_counts (a counter for each warp and bucket) has been zeroed by the CTA.
 // Lanes of the same digit are found by a ballot for each bit of it.
 template<typename Put>
 __device__ __forceinline__ void rank_tile(const uint32_t (&d)[kRounds], uint32_t bits, uint32_t buckets, uint16_t *warp_counts, uint32_t (&rank)[kRounds], Put put) {
     const uint32_t warps = blockDim.x >> 5, lane = threadIdx.x & 31u;
-    const uint32_t words = (warps * buckets + 7) / 8;
-    for (uint32_t i = threadIdx.x; i < words; i += blockDim.x) reinterpret_cast<uint4 *>(warp_counts)[i] = make_uint4(0, 0, 0, 0);
     uint32_t same[kRounds];
 #pragma unroll
     for (uint32_t r = 0; r < kRounds; r++) same[r] = __ballot_sync(0xffffffffu, d[r] != kNone);
@@ -463,6 +462,7 @@ __global__ void __launch_bounds__(kTileThreads) bucket_count_kernel(Keys keys, u
                                                                     uint32_t *__restrict__ counts, uint16_t *__restrict__ ranks, Clear clear) {
     extern __shared__ __align__(16) uint16_t warp_counts[];
     if (blockIdx.x >= tiles) return clear.block(blockIdx.x - tiles);
+    for (uint32_t i = threadIdx.x; i < rank_smem(kTileThreads / 32, buckets) / 16; i += kTileThreads) reinterpret_cast<uint4 *>(warp_counts)[i] = make_uint4(0, 0, 0, 0);
     wait_for_previous();
     const uint32_t first = blockIdx.x * kTile;
     uint32_t d[kRounds], rank[kRounds];
@@ -519,18 +519,19 @@ __global__ void __launch_bounds__(kTileThreads) bucket_place_kernel(Keys keys, u
                                                                     const uint16_t *__restrict__ ranks, To to, Clear clear) {
     extern __shared__ __align__(16) uint32_t base[];   // of each bucket: all items of smaller ones; then, behind, its items in the tiles before
     if (blockIdx.x >= tiles) return clear.block(blockIdx.x - tiles);
-    wait_for_previous();
     const uint32_t stride = count_stride(buckets);
     uint32_t *before = base + stride;
     const uint32_t first = blockIdx.x * kTile;
     uint2 item[kRounds];
     uint32_t rank[kRounds];
+    // the items were there before the launch before this one began; ranks and counts are what it makes
 #pragma unroll
-    for (uint32_t r = 0; r < kRounds; r++) {
-        const uint32_t i = min(first + r * kTileThreads + threadIdx.x, items - 1);
-        item[r] = keys.item(i);
-        rank[r] = ranks[i];
-    }
+    for (uint32_t r = 0; r < kRounds; r++) item[r] = keys.item(min(first + r * kTileThreads + threadIdx.x, items - 1));
+    if (!kScanned)
+        for (uint32_t b = threadIdx.x; b < 2 * stride; b += kTileThreads) base[b] = 0;
+    wait_for_previous();
+#pragma unroll
+    for (uint32_t r = 0; r < kRounds; r++) rank[r] = ranks[min(first + r * kTileThreads + threadIdx.x, items - 1)];
     if constexpr (kScanned) {
         for (uint32_t b = threadIdx.x; b < buckets; b += kTileThreads) {
             base[b] = totals[b];
@@ -539,7 +540,6 @@ __global__ void __launch_bounds__(kTileThreads) bucket_place_kernel(Keys keys, u
     } else {
         // four buckets a thread; where that leaves threads over, groups of them share the tiles
         const uint32_t quads = stride / 4, across = min(quads, kTileThreads), groups = kTileThreads / across, group = threadIdx.x / across;
-        for (uint32_t b = threadIdx.x; b < 2 * stride; b += kTileThreads) base[b] = 0;
         __syncthreads();
         const uint32_t each = (tiles + groups - 1) / groups, t0 = group * each, t1 = min(t0 + each, tiles);
         if (group < groups)

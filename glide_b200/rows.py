@@ -81,8 +81,12 @@ def _flat(name: str, t: torch.Tensor, dim: int) -> torch.Tensor:
         raise TypeError(f"{name}: rows of shape {tuple(t.shape)} and strides {t.stride()} do not lie one stride apart") from None
 
 
+# torch.cuda.current_stream(...).cuda_stream without the 2 us that its object takes, where this torch has it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+
 def _stream(ctx: Context) -> int:
-    return torch._C._cuda_getCurrentRawStream(ctx.device)   # torch.cuda.current_stream(...).cuda_stream without the 2 us of its object
+    return _raw_stream(ctx.device)
 
 
 def lookup_rows(ctx: Context, d_table: torch.Tensor, d_ids: torch.Tensor, scale: float = 1.0, out: torch.Tensor | None = None) -> torch.Tensor:
