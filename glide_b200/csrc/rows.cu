@@ -156,7 +156,7 @@ __device__ __forceinline__ void store(O *p, const float (&f)[V]) {
         __stcg(reinterpret_cast<WordOf<O, H> *>(p + h), w);
     }
 }
-// kWritten: the memory is written in the same launch, each word by the thread that reads it
+// kWritten: the memory is written in the same launch, each word by the thread that reads it, or by the launch before
 template<typename O, int V, bool kWritten = false>
 __device__ __forceinline__ void load(const O *p, float (&f)[V]) {
     constexpr int H = 16 / (int) sizeof(O) < V ? 16 / (int) sizeof(O) : V;
@@ -261,7 +261,8 @@ __global__ void __launch_bounds__(256) lookup_long_kernel(Rows<const T> table, u
 
 // ---- launches that follow one another -----------------------------------------------------------------------------
 // The kernels of one call are launched as programmatic dependents: the next one's CTAs become resident while the last one
-// drains, and wait() holds them until everything before is complete and visible.
+// drains, and wait_for_previous() holds them until everything before is complete and visible. What the launch before wrote was not
+// constant while this one ran, so it is never read through the read-only path (__ldg, const __restrict__): by plain loads or __ldcg.
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_previous() {
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -270,7 +271,7 @@ __device__ __forceinline__ void wait_for_previous() {
 
 template<typename... P, typename... A>
 cudaError_t launch(void (*kernel)(P...), uint64_t grid, uint32_t block, uint32_t smem, cudaStream_t stream, bool dependent, A... args) {
-    if (smem > 48 * 1024) {   // more dynamic shared memory than a kernel gets unasked
+    if (smem > 40 * 1024) {   // with what the kernel declares (8 KB at most), more than the 48 KB that it gets unasked
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem);
         if (e != cudaSuccess) return e;
     }
@@ -515,8 +516,7 @@ __global__ void __launch_bounds__(1024) bucket_scan_kernel(uint32_t *__restrict_
 
 template<typename To, bool kScanned>
 __global__ void __launch_bounds__(kTileThreads) bucket_place_kernel(Keys keys, uint32_t items, Digit digit, uint32_t buckets, uint32_t tiles,
-                                                                    const uint32_t *__restrict__ counts, const uint32_t *__restrict__ totals,
-                                                                    const uint16_t *__restrict__ ranks, To to, Clear clear) {
+                                                                    const uint32_t *counts, const uint32_t *totals, const uint16_t *ranks, To to, Clear clear) {
     extern __shared__ __align__(16) uint32_t base[];   // of each bucket: all items of smaller ones; then, behind, its items in the tiles before
     if (blockIdx.x >= tiles) return clear.block(blockIdx.x - tiles);
     const uint32_t stride = count_stride(buckets);
@@ -531,11 +531,11 @@ __global__ void __launch_bounds__(kTileThreads) bucket_place_kernel(Keys keys, u
         for (uint32_t b = threadIdx.x; b < 2 * stride; b += kTileThreads) base[b] = 0;
     wait_for_previous();
 #pragma unroll
-    for (uint32_t r = 0; r < kRounds; r++) rank[r] = ranks[min(first + r * kTileThreads + threadIdx.x, items - 1)];
+    for (uint32_t r = 0; r < kRounds; r++) rank[r] = __ldcg(ranks + min(first + r * kTileThreads + threadIdx.x, items - 1));
     if constexpr (kScanned) {
         for (uint32_t b = threadIdx.x; b < buckets; b += kTileThreads) {
-            base[b] = totals[b];
-            before[b] = counts[(uint64_t) blockIdx.x * stride + b];
+            base[b] = __ldcg(totals + b);
+            before[b] = __ldcg(counts + (uint64_t) blockIdx.x * stride + b);
         }
     } else {
         // four buckets a thread; where that leaves threads over, groups of them share the tiles
@@ -547,7 +547,7 @@ __global__ void __launch_bounds__(kTileThreads) bucket_place_kernel(Keys keys, u
                 uint4 all = make_uint4(0, 0, 0, 0), mine = all;
 #pragma unroll 16
                 for (uint32_t t = t0; t < t1; t++) {
-                    const uint4 c = __ldg(reinterpret_cast<const uint4 *>(counts + t * stride) + q);
+                    const uint4 c = __ldcg(reinterpret_cast<const uint4 *>(counts + t * stride) + q);
                     all.x += c.x; all.y += c.y; all.z += c.z; all.w += c.w;
                     if (t < blockIdx.x) { mine.x += c.x; mine.y += c.y; mine.z += c.z; mine.w += c.w; }
                 }
@@ -635,7 +635,7 @@ __device__ __forceinline__ void put_grad(const Rows<O> &out, const GradArgs &a, 
 }
 
 // The first of the sorted keys from `lo` on that is not below `key`; the CTA narrows the range by its width at each step.
-__device__ __forceinline__ uint32_t first_not_below(const uint2 *__restrict__ sorted, uint32_t lo, uint32_t hi, uint32_t key) {
+__device__ __forceinline__ uint32_t first_not_below(const uint2 *sorted, uint32_t lo, uint32_t hi, uint32_t key) {
     while (lo < hi) {
         const uint32_t step = (hi - lo + blockDim.x - 1) / blockDim.x;
         const uint64_t i = lo + (uint64_t) threadIdx.x * step;
@@ -734,7 +734,7 @@ __global__ void __launch_bounds__(256, 4) grad_join_kernel(Rows<const T> grad, R
     };
     uint2 next[U];   // items of the batch to come: their rows can be fetched without waiting for them
 #pragma unroll
-    for (int u = 0; u < U; u++) next[u] = __ldg(a.sorted + min((uint32_t) c0 + u, c1 - 1));
+    for (int u = 0; u < U; u++) next[u] = a.sorted[min((uint32_t) c0 + u, c1 - 1)];
     for (uint32_t c = (uint32_t) c0; c < c1; c += U) {
         uint32_t key[U];
         Piece<T, V, true> piece[U];
@@ -744,7 +744,7 @@ __global__ void __launch_bounds__(256, 4) grad_join_kernel(Rows<const T> grad, R
             piece[u] = fetch<V, true>(grad, grad.row(next[u].y), (int32_t) (word * V), a.dim, key[u] < a.n && c + u < c1);
         }
 #pragma unroll
-        for (int u = 0; u < U; u++) next[u] = __ldg(a.sorted + min(c + U + u, c1 - 1));
+        for (int u = 0; u < U; u++) next[u] = a.sorted[min(c + U + u, c1 - 1)];
 #pragma unroll
         for (int u = 0; u < U; u++) {
             if (c + u >= c1) break;
@@ -865,7 +865,7 @@ __global__ void __launch_bounds__(256) grad_fix_kernel(Rows<O> out, GradArgs a, 
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 const uint32_t i = min(s + u, s1 - 1);
-                load<float, V>(a.partial + (2ull * (chunk + i) + (i == 0 ? 1 : 0)) * a.dim + word * V, f[u]);
+                load<float, V, true>(a.partial + (2ull * (chunk + i) + (i == 0 ? 1 : 0)) * a.dim + word * V, f[u]);
             }
 #pragma unroll
             for (int u = 0; u < U; u++) {
@@ -938,7 +938,8 @@ __global__ void __launch_bounds__(256) grad_fix_kernel(Rows<O> out, GradArgs a, 
 // other, takes 138: each row is read eight times.
 template<typename T, int V, int U>
 __global__ void __launch_bounds__(256) dispatch_kernel(Rows<const T> rows, uint32_t dim, uint32_t units, Div words, uint32_t choices,
-                                                       const uint32_t *__restrict__ position, Rows<T> sorted) {
+                                                       const uint32_t *position, Rows<T> sorted) {
+    constexpr int K = 8;   // places that are fetched before a piece goes to any of them
     const uint32_t first = blockIdx.x * (256 * U) + threadIdx.x;
     uint32_t row[U], at[U];
     Piece<T, V, true> piece[U];
@@ -953,10 +954,13 @@ __global__ void __launch_bounds__(256) dispatch_kernel(Rows<const T> rows, uint3
 #pragma unroll
     for (int u = 0; u < U; u++) {
         if (first + u * 256 >= units) break;
-#pragma unroll 4
-        for (uint32_t j = 0; j < choices; j++) {
-            const uint32_t p = position[(uint64_t) row[u] * choices + j];
-            if (p != kNone) __stcg(reinterpret_cast<WordOf<T, V> *>(sorted.row(p) + at[u]), piece[u].a);
+        for (uint32_t j0 = 0; j0 < choices; j0 += K) {
+            uint32_t p[K];
+#pragma unroll
+            for (int j = 0; j < K; j++) p[j] = j0 + j < choices ? position[(uint64_t) row[u] * choices + j0 + j] : kNone;
+#pragma unroll
+            for (int j = 0; j < K; j++)
+                if (p[j] != kNone) __stcg(reinterpret_cast<WordOf<T, V> *>(sorted.row(p[j]) + at[u]), piece[u].a);
         }
     }
 }
@@ -964,7 +968,8 @@ __global__ void __launch_bounds__(256) dispatch_kernel(Rows<const T> rows, uint3
 // The same with a warp a row, for many long rows.
 template<typename T, int V, int U>
 __global__ void __launch_bounds__(256) dispatch_long_kernel(Rows<const T> rows, uint32_t dim, uint32_t count, uint32_t words, uint32_t choices,
-                                                            const uint32_t *__restrict__ position, Rows<T> sorted) {
+                                                            const uint32_t *position, Rows<T> sorted) {
+    constexpr int K = 4;
     wait_for_previous();
     const uint32_t row = blockIdx.x * 8 + (threadIdx.x >> 5);
     if (row >= count) return;
@@ -974,14 +979,18 @@ __global__ void __launch_bounds__(256) dispatch_long_kernel(Rows<const T> rows, 
         Piece<T, V, true> piece[U];
 #pragma unroll
         for (int u = 0; u < U; u++) piece[u] = fetch<V, true>(rows, from, (int32_t) ((c + u * 32) * V), dim, c + u * 32 < words);
-#pragma unroll 2
-        for (uint32_t j = 0; j < choices; j++) {
-            const uint32_t p = position[j];
-            if (p == kNone) continue;
-            T *to = sorted.row(p) + c * V;
+        for (uint32_t j0 = 0; j0 < choices; j0 += K) {
+            uint32_t p[K];
 #pragma unroll
-            for (int u = 0; u < U; u++)
-                if (c + u * 32 < words) __stcg(reinterpret_cast<WordOf<T, V> *>(to + u * 32 * V), piece[u].a);
+            for (int j = 0; j < K; j++) p[j] = j0 + j < choices ? position[j0 + j] : kNone;
+#pragma unroll
+            for (int j = 0; j < K; j++) {
+                if (p[j] == kNone) continue;
+                T *to = sorted.row(p[j]) + c * V;
+#pragma unroll
+                for (int u = 0; u < U; u++)
+                    if (c + u * 32 < words) __stcg(reinterpret_cast<WordOf<T, V> *>(to + u * 32 * V), piece[u].a);
+            }
         }
     }
 }
