@@ -46,7 +46,6 @@ template<> struct Word<16> { using type = uint4; };
 template<> struct Word<8> { using type = uint2; };
 template<> struct Word<4> { using type = uint32_t; };
 template<> struct Word<2> { using type = uint16_t; };
-template<> struct Word<1> { using type = uint8_t; };
 template<typename T, int V> using WordOf = typename Word<(int) sizeof(T) * V>::type;
 
 __device__ __forceinline__ float to_float(float x) { return x; }
@@ -87,10 +86,8 @@ struct Piece<T, V, false> {
             for (int i = 0; i < 6; i++) w[i] = shift & 8u ? w[i + 2] : w[i];
 #pragma unroll
             for (int i = 0; i < 5; i++) w[i] = shift & 4u ? w[i + 1] : w[i];
-            if constexpr (sizeof(T) < 4) {
 #pragma unroll
-                for (int i = 0; i < 4; i++) w[i] = __funnelshift_r(w[i], w[i + 1], (shift & 3u) * 8);
-            }
+            for (int i = 0; i < 4; i++) w[i] = __funnelshift_r(w[i], w[i + 1], (shift & 3u) * 8);
             return make_uint4(w[0], w[1], w[2], w[3]);
         }
     }
@@ -1076,7 +1073,7 @@ __global__ void __launch_bounds__(256) combine_kernel(Rows<const T> sorted, uint
 }
 
 // The same with a warp a row, for many long rows: U of its pieces and those of K of its places are in flight.
-template<typename T, int V, bool kWhole, int K, int U>
+template<typename T, int V, int K, int U>
 __global__ void __launch_bounds__(256) combine_long_kernel(Rows<const T> sorted, uint32_t sorted_rows, uint32_t dim, const uint32_t *__restrict__ position,
                                                            uint32_t choices, const float *__restrict__ weights, uint32_t count, uint32_t words, Rows<T> out) {
     const uint32_t row = blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -1101,12 +1098,12 @@ __global__ void __launch_bounds__(256) combine_long_kernel(Rows<const T> sorted,
             for (int i = 0; i < V; i++) acc[u][i] = 0.0f;
         for (uint32_t j0 = 0; j0 < choices; j0 += K) {
             if (choices > K) places(j0);
-            Piece<T, V, kWhole> y[U][K];
+            Piece<T, V, true> y[U][K];
 #pragma unroll
             for (int u = 0; u < U; u++)
 #pragma unroll
                 for (int j = 0; j < K; j++)
-                    y[u][j] = fetch<V, kWhole>(sorted, sorted.row(p[j]), piece_start<V, kWhole>(to, c + u * 32), dim, p[j] < sorted_rows && c + u * 32 < words);
+                    y[u][j] = fetch<V, true>(sorted, sorted.row(p[j]), (int32_t) ((c + u * 32) * V), dim, p[j] < sorted_rows && c + u * 32 < words);
 #pragma unroll
             for (int j = 0; j < K; j++) {
                 if (p[j] >= sorted_rows) continue;
@@ -1121,7 +1118,7 @@ __global__ void __launch_bounds__(256) combine_long_kernel(Rows<const T> sorted,
         }
 #pragma unroll
         for (int u = 0; u < U; u++)
-            if (c + u * 32 < words) put<V, kWhole>(to, piece_start<V, kWhole>(to, c + u * 32), dim, acc[u]);
+            if (c + u * 32 < words) store<T, V>(to + (c + u * 32) * V, acc[u]);
     }
 }
 
@@ -1236,9 +1233,9 @@ struct OnDevice {
     ~OnDevice() { if (before >= 0) cudaSetDevice(before); }
 };
 
-#define ROWS_CUDA(...)                                                                                      \
+#define ROWS_CUDA(...)                                                                                       \
     do {                                                                                                     \
-        const cudaError_t e_ = (__VA_ARGS__);                                                                     \
+        const cudaError_t e_ = (__VA_ARGS__);                                                                \
         if (e_ != cudaSuccess) return fail(ctx, GLIDE_ERR_CUDA, "%s: %s", __func__, cudaGetErrorString(e_)); \
     } while (0)
 
@@ -1489,6 +1486,12 @@ int glide_lookup_rows_grad(glide_ctx *ctx, const void *d_grad, int row_type, uin
         }));
         return GLIDE_OK;
     }
+    lanes_up_to(32);
+    a.slabs = (uint32_t) ceil_div(a.words, a.lanes);
+    const uint64_t chunks = ceil_div(items, a.chunk), join = ceil_div(chunks * a.slabs * a.lanes, 256), units = (chunks - 1) * a.slabs;
+    // threads are counted in 32 bits, CTAs in 31; nothing has been launched yet
+    ROWS_REQUIRE(join <= 0xffffffu && units <= 0x7fffffffu && join + ceil_div(n, clear_each) <= 0x7fffffffu, GLIDE_ERR_UNSUPPORTED, "lookup_rows_grad: too many values in one call");
+    a.join_blocks = (uint32_t) join;
     const uint64_t share = accumulate || count >= n / 2 ? 0 : kClearShare / row_bytes;
     auto clear = [&]() {
         const Clear c{static_cast<uint8_t *>(d_table_grad) + (uint64_t) cleared * table_grad_stride * bytes_of(grad_type), table_grad_stride * bytes_of(grad_type), row_bytes,
@@ -1510,12 +1513,7 @@ int glide_lookup_rows_grad(glide_ctx *ctx, const void *d_grad, int row_type, uin
     }
     a.sorted = sorted;
     a.clear_from = cleared;
-    lanes_up_to(32);
-    a.slabs = (uint32_t) ceil_div(a.words, a.lanes);
-    const uint64_t zero = accumulate ? 0 : ceil_div(n - cleared, clear_each), chunks = ceil_div(items, a.chunk);
-    const uint64_t join = ceil_div(chunks * a.slabs * a.lanes, 256), units = (chunks - 1) * a.slabs;
-    ROWS_REQUIRE(join <= 0xffffffu && units <= 0x7fffffffu && join + zero <= 0x7fffffffu, GLIDE_ERR_UNSUPPORTED, "lookup_rows_grad: too many values in one call");   // threads are counted in 32 bits
-    a.join_blocks = (uint32_t) join;
+    const uint64_t zero = accumulate ? 0 : ceil_div(n - cleared, clear_each);
     ROWS_CUDA(with_types([&](auto t, auto o, auto wd) {
         using T = decltype(t);
         using O = decltype(o);
@@ -1621,11 +1619,14 @@ int glide_combine_rows(glide_ctx *ctx, const void *d_sorted, int row_type, uint6
         return in_parts(count, words, [&](uint64_t r0, uint32_t rows) {
             const uint32_t units = rows * words;
             auto go = [&](auto k) {
-                constexpr int K = decltype(k)::value, U = !kWhole ? (K <= 2 ? 2 : 1) : in_flight((K <= 2 ? 64 : 128) / K, V * (int) sizeof(T), 8);
-                // with a few choices, of which many may be missing, a thread a piece has too little in flight, whatever the width
-                if (long_rows(rows, words, kWhole && K != 4 && choices > 1 ? V * sizeof t : kWhole ? 8 : 16))
-                    return launch(combine_long_kernel<T, V, kWhole, K, U>, ceil_div(rows, 8), 256, 0, s, false, in.as<const T>(), (uint32_t) sorted_rows, dim, d_position + r0 * choices, choices,
-                                  d_weights_or_null ? d_weights_or_null + r0 * choices : nullptr, rows, words, out.from(r0).as<T>());
+                constexpr int K = decltype(k)::value;
+                // With one choice, or a few of which many may be missing, a thread a piece has too little in flight, whatever the width: 21,701 x 6
+                // rows of 3 KB, two thirds of them missing, 61 us, by a warp a row 48; one choice, 32,081 rows of 4.5 KB, 76 and 56; but
+                // 39,047 x 4 of 5 KB, all there, 143 and 153. Shifted pieces: a thread a piece 65, a warp a row 70 (20,000 x 4 of 2 KB).
+                if constexpr (kWhole)
+                    if (long_rows(rows, words, K == 4 || choices == 1 ? 8 : V * sizeof t))
+                        return launch(combine_long_kernel<T, V, K, in_flight((K <= 2 ? 64 : 128) / K, V * (int) sizeof(T), 8)>, ceil_div(rows, 8), 256, 0, s, false, in.as<const T>(), (uint32_t) sorted_rows,
+                                      dim, d_position + r0 * choices, choices, d_weights_or_null ? d_weights_or_null + r0 * choices : nullptr, rows, words, out.from(r0).as<T>());
                 return launch(combine_kernel<T, V, kWhole, K>, ceil_div(units, 256), 256, 0, s, false, in.as<const T>(), (uint32_t) sorted_rows, dim, d_position + r0 * choices, choices,
                               d_weights_or_null ? d_weights_or_null + r0 * choices : nullptr, units, Div(words), out.from(r0).as<T>());
             };
