@@ -7,8 +7,11 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <map>
+#include <mutex>
 #include <new>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "../../include/glide_b200.h"
@@ -17,6 +20,25 @@
 #include "scan.cuh"
 
 using namespace glide;
+
+cudaError_t glide::allow_shared(const void *kernel, size_t bytes) {
+    static std::mutex mutex;
+    static std::map<std::pair<const void *, int>, size_t> allowed;   // of a kernel on a device
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return e;
+    try {
+        const std::lock_guard<std::mutex> lock(mutex);
+        size_t &most = allowed[{kernel, device}];
+        const size_t wanted = std::max(most, bytes);
+        // set even where it was allowed before: a device that was reset in between has forgotten it
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) wanted);
+        if (e == cudaSuccess) most = wanted;
+        return e;
+    } catch (...) {   // no memory for the entry, or no lock
+        return cudaErrorMemoryAllocation;
+    }
+}
 
 namespace {
 

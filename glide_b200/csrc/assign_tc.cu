@@ -295,7 +295,7 @@ __global__ void __launch_bounds__(128) assign_umma_kernel(const AssignArgs a) {
 
 cudaError_t launch_umma(const AssignArgs &a, cudaStream_t stream) {
     const size_t smem_bytes = (size_t) 3 * kUmmaRows * a.dim * 4 + 2 * kUmmaRows * 4 + kUmmaRows * kCand * 4 + 2 * 8 + 16;
-    cudaError_t e = cudaFuncSetAttribute(assign_umma_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem_bytes);
+    cudaError_t e = allow_shared(assign_umma_kernel, smem_bytes);
     if (e != cudaSuccess) return e;
     assign_umma_kernel<<<(a.n + kUmmaRows - 1) / kUmmaRows, 128, smem_bytes, stream>>>(a);
     return cudaGetLastError();
@@ -500,7 +500,7 @@ cudaError_t launch_umma_tma(const AssignArgs &a, cudaStream_t stream) {
     CUtensorMap tm_points, tm_centroids;
     if (!make_row_map(&tm_points, a.data, a.n, a.dim, kUmmaRows) || !make_row_map(&tm_centroids, a.centroids, a.C, a.dim, kUmmaRows)) return cudaErrorNotSupported;
     const size_t smem_bytes = 1024 + (size_t) 3 * kUmmaRows * a.dim * 4 + 8 * kUmmaRows * 4 + kUmmaRows * kCand * 4 + kUmmaRows * 4 + 8 * 8 + 16;
-    cudaError_t e = cudaFuncSetAttribute(assign_umma_tma_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem_bytes);
+    cudaError_t e = allow_shared(assign_umma_tma_kernel, smem_bytes);
     if (e != cudaSuccess) return e;
     assign_umma_tma_kernel<<<(a.n + kUmmaRows - 1) / kUmmaRows, kTmaThreads, smem_bytes, stream>>>(a, tm_points, tm_centroids);
     return cudaGetLastError();

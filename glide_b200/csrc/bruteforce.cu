@@ -338,8 +338,7 @@ cudaError_t launch_bruteforce(const float *base, uint32_t n, const float *querie
     if (Q == 0) return cudaSuccess;
     if (k == 0 || k > kMaxK || k > n || splits == 0) return cudaErrorInvalidValue;
     const size_t smem_bytes = tile_smem_bytes(k);
-    cudaError_t e = cudaFuncSetAttribute(bruteforce_tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int) smem_bytes);
+    cudaError_t e = allow_shared(bruteforce_tile_kernel, smem_bytes);
     if (e != cudaSuccess) return e;
     const dim3 grid((Q + kQT - 1) / kQT, splits);
     bruteforce_tile_kernel<<<grid, 256, smem_bytes, stream>>>(base, n, queries, Q, dim, k, splits,
@@ -376,11 +375,11 @@ cudaError_t launch_segment_knn(const float *data, uint32_t dim, const uint32_t *
     const size_t smem_bytes = segment_knn_smem_bytes(L);
     cudaError_t e;
     if (L == 32) {
-        e = cudaFuncSetAttribute(segment_knn_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem_bytes);
+        e = allow_shared(segment_knn_kernel<1>, smem_bytes);
         if (e != cudaSuccess) return e;
         segment_knn_kernel<1><<<tile_count, 256, smem_bytes, stream>>>(data, dim, reinterpret_cast<const SegTile *>(d_tiles), out, out_degree, row_base);
     } else {
-        e = cudaFuncSetAttribute(segment_knn_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem_bytes);
+        e = allow_shared(segment_knn_kernel<2>, smem_bytes);
         if (e != cudaSuccess) return e;
         segment_knn_kernel<2><<<tile_count, 256, smem_bytes, stream>>>(data, dim, reinterpret_cast<const SegTile *>(d_tiles), out, out_degree, row_base);
     }

@@ -340,7 +340,7 @@ cudaError_t launch_build_t(const BuildDev &d, uint32_t warps_per_cta, size_t sme
     if constexpr (NC == 2) kernel = rows_fit_lanes(d.a.dim) ? build_kernel<NB, NC, LANES, DimOf<true>> : build_kernel<NB, NC, LANES, DimOf<false>>;
     else kernel = build_kernel<NB, NC, LANES, uint32_t>;   // adjacency rows above 64 entries
     if (smem_bytes > 48 * 1024) {
-        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem_bytes);
+        cudaError_t e = allow_shared(kernel, smem_bytes);
         if (e != cudaSuccess) return e;
     }
     const uint32_t grid = (d.a.count + warps_per_cta - 1) / warps_per_cta;
@@ -614,7 +614,7 @@ cudaError_t launch_reverse(const ReverseArgs &a, cudaStream_t stream) {
     const uint32_t warps = 8;
     const size_t smem_bytes = (size_t) warps * (5 * max_degree + 64) * 4;
     if (smem_bytes > 48 * 1024) {
-        e = cudaFuncSetAttribute(reverse_insert_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem_bytes);
+        e = allow_shared(reverse_insert_kernel, smem_bytes);
         if (e != cudaSuccess) return e;
     }
     reverse_insert_kernel<<<(a.num + warps - 1) / warps, warps * 32, smem_bytes, stream>>>(

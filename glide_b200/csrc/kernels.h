@@ -14,6 +14,12 @@ struct BeamParamsHost {
     uint32_t beam, max_iterations, min_iterations, hash_bit, hash_reset_interval;
 };
 
+// How much dynamic shared memory a launch of a kernel may ask for is an attribute that the kernel has on a device, for all threads of the
+// process. allow_shared raises it to `bytes` and never lowers it: set to what one thread's call needs, it would take away what another
+// thread has set and is about to launch with. (api.cu)
+cudaError_t allow_shared(const void *kernel, size_t bytes);
+template<typename... P> cudaError_t allow_shared(void (*kernel)(P...), size_t bytes) { return allow_shared(reinterpret_cast<const void *>(kernel), bytes); }
+
 // ---- search.cu -----------------------------------------------------------
 // One partition of the large path as the device sees it (local ids; map: local id -> original id).
 struct PartitionRef {

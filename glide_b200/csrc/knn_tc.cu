@@ -466,11 +466,11 @@ cudaError_t run(const float *data, uint64_t rows_total, uint32_t dim, const std:
     if (e != cudaSuccess) return e;
     row_norms_kernel<<<(unsigned) ((rows_total * 32 + 255) / 256), 256, 0, stream>>>(data, rows_total, dim, norms);
     const size_t smem_main = 1024 + (size_t) 3 * kRows * dim * 4 + (kEpiWarps * kCols + kRows) * 4 + (1 + 2 * kStages + 5) * 8 + 16;
-    if ((e = cudaFuncSetAttribute(knn_umma_kernel<NL>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem_main)) != cudaSuccess) return e;
+    if ((e = allow_shared(knn_umma_kernel<NL>, smem_main)) != cudaSuccess) return e;
     const uint32_t rr_warps = 8;
     const size_t smem_rr = (size_t) rr_warps * (dim_pad4(dim) + 2 * Sizes<NL>::keep) * 4;
     if (smem_rr > 48 * 1024 &&
-        (e = cudaFuncSetAttribute(knn_rerank_kernel<NL>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem_rr)) != cudaSuccess) return e;
+        (e = allow_shared(knn_rerank_kernel<NL>, smem_rr)) != cudaSuccess) return e;
     KnnTcArgs a{data, dim, rows_total, norms, d_tiles, cand, cand_count, gmin, fail_flag};
     for (size_t first = 0; first < tiles.size(); first += kMaxCtasPerLaunch) {
         const uint32_t n = (uint32_t) std::min<size_t>(kMaxCtasPerLaunch, tiles.size() - first);

@@ -421,10 +421,10 @@ cudaError_t run_nn_descent(const NndArgs &a, cudaStream_t stream) {
     const uint32_t wgrid = (a.rows + warps - 1) / warps;
     const size_t init_smem = (size_t) warps * (dim_pad4(a.dim) + 2 * a.K) * 4;
     if (a.K == 32) {
-        if (init_smem > 48 * 1024) cudaFuncSetAttribute(nnd_init_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) init_smem);
+        if (init_smem > 48 * 1024) allow_shared(nnd_init_kernel<1>, init_smem);
         nnd_init_kernel<1><<<wgrid, warps * 32, init_smem, stream>>>(d);
     } else {
-        if (init_smem > 48 * 1024) cudaFuncSetAttribute(nnd_init_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) init_smem);
+        if (init_smem > 48 * 1024) allow_shared(nnd_init_kernel<2>, init_smem);
         nnd_init_kernel<2><<<wgrid, warps * 32, init_smem, stream>>>(d);
     }
     if ((e = cudaGetLastError()) != cudaSuccess) return e;

@@ -576,7 +576,7 @@ cudaError_t launch_assign(const AssignArgs &a, cudaStream_t stream, uint32_t *la
     while (warps > 1 && (size_t) strip_words * 4 * warps > 96 * 1024) warps >>= 1;
     const size_t smem_bytes = (size_t) strip_words * 4 * warps;
     if (smem_bytes > 48 * 1024) {
-        cudaError_t e = cudaFuncSetAttribute(assign_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem_bytes);
+        cudaError_t e = allow_shared(assign_kernel, smem_bytes);
         if (e != cudaSuccess) return e;
     }
     // the tiled kernel settles every point whose nearest centroid is unique; the warp-per-point
@@ -733,7 +733,7 @@ static cudaError_t launch_farthest_first_persistent(const float *sample, uint32_
     const void *kernel = ch == 1 ? (const void *) ff_persistent_kernel<1> : ch == 2 ? (const void *) ff_persistent_kernel<2>
                        : ch == 3 ? (const void *) ff_persistent_kernel<3> : ch == 4 ? (const void *) ff_persistent_kernel<4>
                                                                                      : (const void *) ff_persistent_kernel<0>;
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem);
+    e = allow_shared(kernel, smem);
     int per_sm = 0;
     if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, (int) kFfThreads, smem);
     if (e != cudaSuccess) return e;

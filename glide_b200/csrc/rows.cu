@@ -269,7 +269,7 @@ __device__ __forceinline__ void wait_for_previous() {
 template<typename... P, typename... A>
 cudaError_t launch(void (*kernel)(P...), uint64_t grid, uint32_t block, uint32_t smem, cudaStream_t stream, bool dependent, A... args) {
     if (smem > 40 * 1024) {   // with what the kernel declares (8 KB at most), more than the 48 KB that it gets unasked
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem);
+        const cudaError_t e = allow_shared(kernel, smem);
         if (e != cudaSuccess) return e;
     }
     cudaLaunchAttribute attr{};

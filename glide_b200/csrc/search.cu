@@ -74,7 +74,7 @@ cudaError_t launch_search_t(const SearchDev &d, uint32_t warps_per_cta, size_t s
     if constexpr (NC == 2) kernel = rows_fit_lanes(d.a.dim) ? search_instance<NB, NC, LANES, DimOf<true>>(d.a) : search_instance<NB, NC, LANES, DimOf<false>>(d.a);
     else kernel = search_instance<NB, NC, LANES, uint32_t>(d.a);   // adjacency rows above 64 entries
     if (smem_bytes > 48 * 1024) {
-        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem_bytes);
+        cudaError_t e = allow_shared(kernel, smem_bytes);
         if (e != cudaSuccess) return e;
     }
     uint32_t grid = 0;
@@ -152,8 +152,7 @@ cudaError_t launch_select_segments(const SelectSegmentArgs &a, cudaStream_t stre
     const uint32_t warps = 4;
     const size_t smem_bytes = (size_t) strip_words * 4 * warps;
     if (smem_bytes > 48 * 1024) {
-        cudaError_t e = cudaFuncSetAttribute(select_segment_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             (int) smem_bytes);
+        cudaError_t e = allow_shared(select_segment_kernel, smem_bytes);
         if (e != cudaSuccess) return e;
     }
     select_segment_kernel<<<(a.Q + warps - 1) / warps, warps * 32, smem_bytes, stream>>>(a, max_centroid, strip_words);

@@ -49,7 +49,7 @@ cudaError_t launch_team_t(const SearchDev &given, size_t smem_bytes, int sms, cu
     SearchDev d = given;
     void (*kernel)(const SearchDev) = rows_fit_lanes(d.a.dim) ? team_instance<NB, NC, LANES, DimOf<true>>(d.a) : team_instance<NB, NC, LANES, DimOf<false>>(d.a);
     if (smem_bytes > 48 * 1024) {
-        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem_bytes);
+        cudaError_t e = allow_shared(kernel, smem_bytes);
         if (e != cudaSuccess) return e;
     }
     const uint32_t warps = team_warps(reinterpret_cast<const void *>(kernel), d.a, smem_bytes, sms);

@@ -753,10 +753,10 @@ cudaError_t launch_truth_tc(const TcPasses &passes, const float *base, uint32_t 
     a.stages = ring_stages(a.kblocks);
     a.norms = norms; a.thr = thr; a.gmin = gmin; a.count = count; a.cand = cand; a.gave_up = bad.gave_up;
     const size_t smem = umma_smem(a.stages);
-    if ((e = cudaFuncSetAttribute(truth_umma_kernel<true, CUtensorMap>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem)) != cudaSuccess) return e;
-    if ((e = cudaFuncSetAttribute(truth_umma_kernel<false, CUtensorMap>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem)) != cudaSuccess) return e;
+    if ((e = allow_shared(truth_umma_kernel<true, CUtensorMap>, smem)) != cudaSuccess) return e;
+    if ((e = allow_shared(truth_umma_kernel<false, CUtensorMap>, smem)) != cudaSuccess) return e;
     const size_t rr_smem = 4096 * 8 + (size_t) p.pitch * 4;
-    if (rr_smem > 48 * 1024 && (e = cudaFuncSetAttribute(truth_rerank_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) rr_smem)) != cudaSuccess) return e;
+    if (rr_smem > 48 * 1024 && (e = allow_shared(truth_rerank_kernel, rr_smem)) != cudaSuccess) return e;
 
     for (uint32_t qa = 0; qa < Q; qa += p.qb) {
         const uint32_t nq = Q - qa < p.qb ? Q - qa : p.qb;
@@ -929,8 +929,8 @@ cudaError_t launch_segment_tc(const TcPasses &passes, const float *data, uint32_
     a.fold = 1;
     a.norms = at(p.norms); a.thr = at(p.thr); a.gmin = at(p.gmin); a.count = count; a.cand = cand; a.gave_up = bad.gave_up;
     const size_t smem = umma_smem(a.stages), rr_smem = (size_t) kSegCap * 8 + (size_t) p.pitch * 4;
-    if ((e = cudaFuncSetAttribute(truth_umma_kernel<true, SampleMaps>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem)) != cudaSuccess) return e;
-    if ((e = cudaFuncSetAttribute(truth_umma_kernel<false, CUtensorMap>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem)) != cudaSuccess) return e;
+    if ((e = allow_shared(truth_umma_kernel<true, SampleMaps>, smem)) != cudaSuccess) return e;
+    if ((e = allow_shared(truth_umma_kernel<false, CUtensorMap>, smem)) != cudaSuccess) return e;
     for (const SegChunk &c : p.chunks) {
         // (a grid's second dimension ends at 65,535)
         for (uint32_t t = 0; centred && t < c.tiles; t += 32768)
