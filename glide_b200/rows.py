@@ -134,8 +134,9 @@ def lookup_rows_grad(ctx: Context, d_grad: torch.Tensor, d_ids: torch.Tensor, nu
 def dispatch_rows(ctx: Context, d_rows: torch.Tensor, d_choice: torch.Tensor, partitions: int, out: torch.Tensor | None = None) -> Dispatched:
     """Rows sorted by the partitions that they chose: d_choice [rows, choices] holds up to 128 partitions for each row (the ids of
     ``bruteforce_knn(ctx, d_centroids, d_rows, k)``, or a router's), -1 for none. Pairs of a row and a choice are ordered by partition,
-    then row, then choice. out: where the sorted rows go; rows behind the last place taken are left as they were. The gradient
-    with respect to d_rows is ``dispatch_rows_grad``."""
+    then row, then choice. out: where the sorted rows go; rows behind the last place taken (d_segment_start[partitions]) are left as they
+    were. Without `out` they are undefined, any bits: a product that takes in all rows, not partition by partition, wants
+    out=torch.zeros(...). The gradient with respect to d_rows is ``dispatch_rows_grad``."""
     rows, kind, stride = _matrix(ctx, "d_rows", d_rows)
     count, dim = d_rows.shape
     choice = _whole(ctx, "d_choice", d_choice, torch.int32)
@@ -188,9 +189,10 @@ def dispatch_rows_grad(ctx: Context, d_grad_sorted: torch.Tensor, d_position: to
 
 def combine_rows_grad(ctx: Context, d_grad: torch.Tensor, d_sorted: torch.Tensor, d_position: torch.Tensor,
                       d_weights: torch.Tensor | None = None, out: torch.Tensor | None = None):
-    """The gradients of ``combine_rows`` with respect to its sorted rows (weight * d_grad at each place; rows that no position names
-    are left as they were) and to its weights (the products of d_grad with the sorted rows, fp32, 0 for a place of -1).
-    out: where the gradient of the sorted rows goes. Places have to be distinct, as ``dispatch_rows`` makes them."""
+    """The gradients of ``combine_rows`` with respect to its sorted rows (weight * d_grad at each place, zeros for rows that no position
+    names) and to its weights (the products of d_grad with the sorted rows, fp32, 0 for a place of -1). out: where the gradient of
+    the sorted rows goes; rows of it that no position names are left as they were, which saves clearing it for every call.
+    Places have to be distinct, as ``dispatch_rows`` makes them."""
     grad, kind, grad_stride = _matrix(ctx, "d_grad", d_grad)
     data, data_kind, stride = _matrix(ctx, "d_sorted", d_sorted)
     sorted_rows, dim = d_sorted.shape
@@ -202,7 +204,7 @@ def combine_rows_grad(ctx: Context, d_grad: torch.Tensor, d_sorted: torch.Tensor
         raise ValueError(f"d_grad must be {d_sorted.dtype} of shape {(count, dim)}, got {d_grad.dtype} of {tuple(d_grad.shape)}")
     weights = None if d_weights is None else _whole(ctx, "d_weights", d_weights, torch.float32, shape)
     if out is None:
-        out = d_sorted.new_empty((sorted_rows, dim))
+        out = d_sorted.new_zeros((sorted_rows, dim))
     else:
         _check_result(ctx, out, (sorted_rows, dim), d_sorted.dtype)
     to, _, to_stride = _matrix(ctx, "out", out)

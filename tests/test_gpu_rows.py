@@ -411,6 +411,26 @@ def test_combine_grad(gpu_ctx, dtype, weighted, count, dim, choices, empty):
     assert (got_w[~there] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("count,dim,choices,empty", [(0, 40, 3, 0.0), (1, 24, 1, 1.0), (64, 512, 2, 0.4), (700, 33, 8, 0.3), (3000, 128, 2, 0.5)])
+def test_combine_grad_makes_zeros_of_rows_without_a_place(gpu_ctx, dtype, count, dim, choices, empty):
+    """A result that the call itself makes, in memory that held NaN before; with more sorted rows than pairs, too."""
+    data, position, weights = _combine_case(dtype, count, dim, choices, empty, 56)
+    grad = _randn((count, dim), dtype, 59)
+    for more in (0, 5):
+        data = torch.cat([data, _randn((more, dim), dtype, 58)])
+        torch.full(data.shape, float("nan"), dtype=dtype, device="cuda")      # goes back to the allocator, which gives it out again
+        got, _ = rows.combine_rows_grad(gpu_ctx, grad, data, position, weights)
+        there = position >= 0
+        at = position[there].long()
+        want = torch.zeros(data.shape, dtype=torch.float64, device="cuda")
+        want[at] = (grad.double()[:, None] * weights[..., None].double())[there]
+        _close(got, want, want.abs() * (U + _half(dtype)) + _floor(dtype))
+        rest = torch.ones(data.shape[0], dtype=torch.bool, device="cuda")
+        rest[at] = False
+        assert (got[rest] == 0).all()
+
+
 def test_combine_leaves_out_what_has_no_place_whatever_it_would_hold(gpu_ctx):
     data = _randn((6, 40), torch.float32, 50)
     data[5] = float("nan")
