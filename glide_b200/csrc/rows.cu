@@ -260,6 +260,8 @@ __global__ void __launch_bounds__(256) lookup_long_kernel(Rows<const T> table, u
 // The kernels of one call are launched as programmatic dependents: the next one's CTAs become resident while the last one
 // drains, and wait_for_previous() holds them until everything before is complete and visible. What the launch before wrote was not
 // constant while this one ran, so it is never read through the read-only path (__ldg, const __restrict__): by plain loads or __ldcg.
+// Before its wait a kernel reads the call's inputs and nothing that the call has made, however many launches ago: a wait is what makes that
+// visible. CTAs that only clear rows of the result wait for nothing; every launch has others that do, so its end is the end of all before.
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_previous() {
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -521,12 +523,18 @@ __global__ void __launch_bounds__(kTileThreads) bucket_place_kernel(Keys keys, u
     const uint32_t first = blockIdx.x * kTile;
     uint2 item[kRounds];
     uint32_t rank[kRounds];
-    // the items were there before the launch before this one began; ranks and counts are what it makes
+    const bool given = keys.items == nullptr;   // by the caller: they need not wait, as items that an earlier pass has placed do
+    if (given) {
 #pragma unroll
-    for (uint32_t r = 0; r < kRounds; r++) item[r] = keys.item(min(first + r * kTileThreads + threadIdx.x, items - 1));
+        for (uint32_t r = 0; r < kRounds; r++) item[r] = keys.item(min(first + r * kTileThreads + threadIdx.x, items - 1));
+    }
     if (!kScanned)
         for (uint32_t b = threadIdx.x; b < 2 * stride; b += kTileThreads) base[b] = 0;
     wait_for_previous();
+    if (!given) {
+#pragma unroll
+        for (uint32_t r = 0; r < kRounds; r++) item[r] = __ldcg(keys.items + min(first + r * kTileThreads + threadIdx.x, items - 1));
+    }
 #pragma unroll
     for (uint32_t r = 0; r < kRounds; r++) rank[r] = __ldcg(ranks + min(first + r * kTileThreads + threadIdx.x, items - 1));
     if constexpr (kScanned) {

@@ -192,6 +192,26 @@ def test_lookup_grad_sorts_every_size(gpu_ctx, count, n):
     assert torch.equal(rows.lookup_rows_grad(gpu_ctx, grad, ids, n).double(), want)
 
 
+@pytest.mark.parametrize("count,n", [(5000, 1_000_000), (200_000, 1_000_000), (5000, 5_000_000), (200_000, 5_000_000)])
+def test_lookup_grad_sorts_in_a_workspace_that_earlier_calls_have_used(gpu_ctx, count, n):
+    """Two and three passes, two and three launches each, one call behind the other in the same workspace with other ids: what a pass reads is
+    what the pass before it has placed in the same call, not in an earlier one."""
+    lib, dim, calls = gpu_ctx.lib, 2, 20
+    need = lib.glide_lookup_rows_grad_workspace(n, dim, count)
+    scratch = torch.empty(need, dtype=torch.uint8, device="cuda")
+    ids = [_ids((count,), n, 140 + i, 0.02) for i in range(calls)]
+    grad = torch.randint(-50, 50, (count, dim), generator=_gen(139), device="cuda").float()
+    out = [torch.full((n, dim), float("nan"), device="cuda") for _ in range(calls)]
+    stream = torch.cuda.current_stream().cuda_stream
+    for i in range(calls):
+        gpu_ctx.check(lib.glide_lookup_rows_grad(gpu_ctx.handle, grad.data_ptr(), 0, dim, ids[i].data_ptr(), count, 1.0, out[i].data_ptr(), 0, n, dim, dim, 0,
+                                                 scratch.data_ptr(), need, stream))
+    for i in range(calls):
+        there = ids[i] >= 0
+        want = torch.zeros((n, dim), dtype=torch.float64, device="cuda").index_add_(0, ids[i][there].long(), grad[there].double())
+        assert torch.equal(out[i].double(), want)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_lookup_grad_accumulates_and_leaves_other_rows(gpu_ctx, dtype):
     base = _randn((500, 72), dtype, 16)
