@@ -518,11 +518,16 @@ class GLIDE:
                                             int(self.metric), _ptr(h_ids), _ptr(h_dists)))
         return h_ids, h_dists
 
-    def lookup(self, d_ids: torch.Tensor, scale: float = 1.0, out: torch.Tensor | None = None) -> torch.Tensor:
-        """The rows of the index with these ids (an int32 tensor of uint32 patterns on the device, such as ``search`` and
-        ``bruteforce_knn`` of this module return), times `scale`: d_ids.shape + (dim,), zeros for 0xffffffff. Ordered on torch's
-        current stream, without a wait (``rows.lookup_rows``)."""
+    def lookup(self, d_ids: torch.Tensor | np.ndarray, scale: float = 1.0, out: torch.Tensor | None = None) -> torch.Tensor:
+        """The rows of the index with these ids, times `scale`, on the device: d_ids.shape + (dim,), zeros for 0xffffffff. d_ids: an int32
+        tensor of uint32 patterns on the device, such as ``search`` and ``bruteforce_knn`` of this module return, or an array on the host,
+        such as this class's ``search`` and ``search_host`` do, which is copied to the device first. Ordered on torch's current stream;
+        with ids on the device there is no wait, and the call can be captured (``rows.lookup_rows``)."""
         from . import rows
+        if isinstance(d_ids, (np.ndarray, np.generic)):
+            if d_ids.dtype not in (np.uint32, np.int32):
+                raise TypeError(f"d_ids must be uint32 or int32, got {d_ids.dtype}")
+            d_ids = from_u32(self.ctx, np.ascontiguousarray(d_ids).view(np.uint32)).reshape(d_ids.shape)
         return rows.lookup_rows(self.ctx, self.d_data, d_ids, scale, out)
 
     def search_pipe(self, max_queries: int, max_top_k: int, depth: int = 3) -> "SearchPipe":

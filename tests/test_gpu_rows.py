@@ -554,6 +554,28 @@ def test_a_search_a_lookup_and_the_gradient_of_the_rows_found(gpu_ctx):
     assert torch.equal(got, want)
 
 
+def test_an_index_looks_up_what_its_own_search_returned(gpu_ctx):
+    """Arrays on the host, of ``search`` and of ``search_host``: with places that a search leaves unfilled, in any shape and order."""
+    from glide_b200.params import SearchParameter
+    g = torch.Generator().manual_seed(86)
+    data, queries = torch.rand((500, 24), generator=g), torch.rand((9, 24), generator=g)
+    index = api.GLIDE(gpu_ctx, 32, data, data[:2])
+    index.load(torch.randint(0, 500, (500, 32), generator=g).numpy().astype(np.uint32), np.array([3, 77], np.uint32))
+    param = SearchParameter(top_k=10, beam=32).derive(32)
+    ids, _, _ = index.search(param, queries.cuda())
+    host_ids, _ = index.search_host(param, queries.numpy())
+    assert isinstance(ids, np.ndarray) and np.array_equal(ids, host_ids)
+    ids[4, 7:] = api.INVALID
+    want = torch.cat([data, torch.zeros((1, 24))])[torch.from_numpy(np.minimum(ids, 500).astype(np.int64))].cuda()
+    assert torch.equal(index.lookup(ids), want) and torch.equal(index.lookup(ids, 2.0), want * 2)
+    assert torch.equal(index.lookup(ids.view(np.int32)), want)
+    assert torch.equal(index.lookup(ids.T[::-1, 1:]), want.transpose(0, 1).flip(0)[:, 1:])
+    assert torch.equal(index.lookup(ids[0, 0].reshape(())), want[0, 0]) and index.lookup(ids[:0]).shape == (0, 10, 24)
+    for bad in (ids.astype(np.int64), ids.astype(np.float32), ids.tolist()):
+        with pytest.raises(TypeError):
+            index.lookup(bad)
+
+
 def test_calls_run_on_the_current_stream(gpu_ctx):
     """Two streams work at once, each on what its own earlier work leaves behind, without a wait on the host between."""
     streams = [torch.cuda.Stream(), torch.cuda.Stream()]
