@@ -153,14 +153,13 @@ __device__ __forceinline__ void store(O *p, const float (&f)[V]) {
         __stcg(reinterpret_cast<WordOf<O, H> *>(p + h), w);
     }
 }
-// kWritten: the memory is written in the same launch, each word by the thread that reads it, or by the launch before
-template<typename O, int V, bool kWritten = false>
+// Of memory that is written in the same launch, each word by the thread that reads it, or by a launch of the same call
+template<typename O, int V>
 __device__ __forceinline__ void load(const O *p, float (&f)[V]) {
     constexpr int H = 16 / (int) sizeof(O) < V ? 16 / (int) sizeof(O) : V;
 #pragma unroll
     for (int h = 0; h < V; h += H) {
-        const auto *from = reinterpret_cast<const WordOf<O, H> *>(p + h);
-        const WordOf<O, H> w = kWritten ? __ldcg(from) : __ldg(from);
+        const WordOf<O, H> w = __ldcg(reinterpret_cast<const WordOf<O, H> *>(p + h));
         O t[H];
         memcpy(t, &w, sizeof w);
 #pragma unroll
@@ -632,7 +631,7 @@ __device__ __forceinline__ void put_grad(const Rows<O> &out, const GradArgs &a, 
     for (int i = 0; i < V; i++) acc[i] *= a.scale;
     if (a.accumulate) {
         float old[V];
-        load<O, V, true>(p, old);
+        load<O, V>(p, old);
 #pragma unroll
         for (int i = 0; i < V; i++) acc[i] += old[i];
     }
@@ -870,7 +869,7 @@ __global__ void __launch_bounds__(256) grad_fix_kernel(Rows<O> out, GradArgs a, 
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 const uint32_t i = min(s + u, s1 - 1);
-                load<float, V, true>(a.partial + (2ull * (chunk + i) + (i == 0 ? 1 : 0)) * a.dim + word * V, f[u]);
+                load<float, V>(a.partial + (2ull * (chunk + i) + (i == 0 ? 1 : 0)) * a.dim + word * V, f[u]);
             }
 #pragma unroll
             for (int u = 0; u < U; u++) {
@@ -1527,7 +1526,7 @@ int glide_lookup_rows_grad(glide_ctx *ctx, const void *d_grad, int row_type, uin
         using O = decltype(o);
         constexpr int V = decltype(wd)::value;
         const cudaError_t e = launch(grad_join_kernel<T, O, V>, join + zero, 256, 0, s, true, in.as<const T>(), out.as<O>(), a);
-        if (e != cudaSuccess || units == 0) return e;
+        if (e != cudaSuccess) return e;   // more than kFewIds ids are more than one chunk, so that units is not 0
         return launch(grad_fix_kernel<O, V>, ceil_div(units, 8), 256, 0, s, true, out.as<O>(), a, (uint32_t) units);
     }));
     return GLIDE_OK;
