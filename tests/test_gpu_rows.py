@@ -226,6 +226,101 @@ def test_lookup_grad_accumulates_and_leaves_other_rows(gpu_ctx, dtype):
     _close(out[touched], want[touched], ((terms + 3) * U * (size + base.double().abs()) + want.abs() * _half(dtype) + _floor(dtype))[touched])
 
 
+def _often(count, n, seed):
+    """Ids of which half are one and the same (a run over many chunks of the sorted list), an eighth another, the others any."""
+    ids, which = _ids((count,), n, seed, 0.05), torch.rand((count,), generator=_gen(seed + 1), device="cuda")
+    return torch.where(which < 0.5, n // 2, torch.where(which < 0.625, n - 2, ids)).int()
+
+
+def _bits(t):
+    return t.view(torch.int32 if t.dtype == torch.float32 else torch.int16)
+
+
+@pytest.mark.parametrize("dtype,out_type", [(t, t) for t in TYPES] + [(torch.float16, torch.float32), (torch.bfloat16, torch.float32)])
+@pytest.mark.parametrize("count,n", [(1024, 300), (1025, 300), (2000, 5000), (6000, 40), (6000, 70_000), (30_000, 900), (30_000, 20_011)])
+@pytest.mark.parametrize("dim,stride,offset", [(1, 1, 0), (33, 40, 1), (72, 72, 0), (520, 528, 8)])
+def test_lookup_grad_accumulates_many_ids(gpu_ctx, dtype, out_type, count, n, dim, stride, offset):
+    """Whole numbers: exact sums, rounded once with what was there. Rows that no id names, and what lies between the rows, hold NaN and keep it."""
+    ids = _often(count, n - 1, 150)
+    grad = torch.randint(-3, 4, (count, dim), generator=_gen(152), device="cuda").to(dtype)
+    out, whole = _strided((n, dim), out_type, 153, stride, offset)
+    whole.fill_(float("nan"))
+    there = ids >= 0
+    named = torch.zeros(n, dtype=torch.bool, device="cuda")
+    named[ids[there].long()] = True
+    base = torch.randint(-60, 61, (n, dim), generator=_gen(154), device="cuda").to(out_type)
+    out[named] = base[named]
+    before = whole.clone()
+    want = base.double().index_add_(0, ids[there].long(), 2 * grad[there].double())
+    assert rows.lookup_rows_grad(gpu_ctx, grad, ids, n, 2.0, out=out, accumulate=True) is out
+    assert torch.equal(out[named], want.to(out_type)[named])
+    assert not named[n - 1] and out[~named].isnan().all()
+    mask = torch.zeros_like(whole, dtype=torch.bool)
+    mask.as_strided((n, dim), (stride, 1), offset).fill_(True)
+    assert torch.equal(_bits(whole)[~mask], _bits(before)[~mask])
+
+
+def test_lookup_grad_accumulates_at_every_replay(gpu_ctx):
+    ids = [_often(count, 3000, 155 + count) for count in (500, 2500, 9000)]
+    grad = torch.randint(-3, 4, (9000, 40), generator=_gen(160), device="cuda").float()
+    out = torch.zeros((3000, 40), device="cuda")
+
+    def step():
+        for i in ids:
+            rows.lookup_rows_grad(gpu_ctx, grad[:i.numel()], i, 3000, out=out, accumulate=True)
+    step()
+    torch.cuda.synchronize()
+    once = out.clone()
+    assert once.abs().max() > 0
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        step()
+    for _ in range(3):
+        g.replay()
+    assert torch.equal(out, once * 4)
+    del g
+
+
+@pytest.mark.parametrize("count,n,dtype,out_type,dim,stride,offset", [
+    (5000, 1_000_003, torch.float32, torch.float32, 100, 100, 0),               # two launches a pass
+    (70_000, 1_000_003, torch.float32, torch.float32, 100, 100, 0),             # three, each beside 48 MB that it clears, the rest by the join
+    (70_000, 1_000_003, torch.bfloat16, torch.bfloat16, 201, 201, 3),           # rows of no whole words
+    (140_000, 1_200_001, torch.bfloat16, torch.float32, 72, 80, 4),             # rows apart from one another
+    (140_000, 600_000, torch.float16, torch.float16, 24, 24, 0),                # all cleared beside the sort
+    (70_000, 4_300_000, torch.float16, torch.float16, 40, 41, 1),               # three passes
+    (140_000, 4_300_000, torch.float32, torch.float32, 4, 4, 0)])
+def test_lookup_grad_clears_large_tables(gpu_ctx, count, n, dtype, out_type, dim, stride, offset):
+    """Every row that no id names is cleared, by whichever launch, and what lies between the rows is left alone."""
+    out, whole = _strided((n, dim), out_type, 161, stride, offset)
+    whole.fill_(float("nan"))
+    ids = _ids((count,), n, 162)
+    grad = torch.randint(-3, 4, (count, dim), generator=_gen(163), device="cuda").to(dtype)
+    rows.lookup_rows_grad(gpu_ctx, grad, ids, n, out=out)
+    there = ids >= 0
+    want = torch.zeros((n, dim), device="cuda").index_add_(0, ids[there].long(), grad[there].float())     # whole numbers: exact
+    assert torch.equal(out, want.to(out_type))
+    if stride != dim:
+        mask = torch.zeros_like(whole, dtype=torch.bool)
+        mask.as_strided((n, dim), (stride, 1), offset).fill_(True)
+        assert whole[~mask].isnan().all()
+
+
+def test_lookup_grad_clears_rows_whose_offsets_pass_32_bits(gpu_ctx):
+    n, dim = 2_100_000, 2_048      # 4.3e9 values
+    out = torch.full((n, dim), 7.0, dtype=torch.float16, device="cuda")
+    for count in (5, 3000, 9000):
+        ids = torch.cat([torch.tensor([n - 1, 0, 2_097_152, 1_048_576, n - 2], dtype=torch.int32, device="cuda"), _ids((count - 5,), n, 164)])
+        grad = torch.randint(-3, 4, (count, dim), generator=_gen(165), device="cuda").half()
+        rows.lookup_rows_grad(gpu_ctx, grad, ids, n, out=out)
+        there = ids >= 0
+        which, back = torch.unique(ids[there].long(), return_inverse=True)
+        want = torch.zeros((which.numel(), dim), device="cuda").index_add_(0, back, grad[there].float())
+        assert torch.equal(out[which].float(), want)
+        out[which] = 0
+        assert all(not out[a:a + 100_000].any() for a in range(0, n, 100_000))
+        out.fill_(7.0)
+
+
 def test_lookup_grad_empty_places_take_no_part_whatever_they_hold(gpu_ctx):
     grad = _randn((40, 24), torch.float32, 19)
     ids = _ids((40,), 9, 20, 0.3)
@@ -464,6 +559,46 @@ def test_combine_leaves_out_what_has_no_place_whatever_it_would_hold(gpu_ctx):
     _, got_w = rows.combine_rows_grad(gpu_ctx, grad, data, position, weights, out=keep)
     assert got_w[0, 1] == 0 and (got_w[1] == 0).all() and got_w[0, 0].isnan()
     assert keep[:3].isnan().all() and (keep[3:] == 1).all()
+
+
+@pytest.mark.parametrize("count,dim,choices", [(40, 64, 2), (900, 600, 9), (3000, 96, 8)])
+def test_combine_grad_without_the_gradient_of_the_weights(gpu_ctx, count, dim, choices):
+    """The C entry point takes null for it (and null for the weights): the gradient of the sorted rows is the same."""
+    data, position, weights = _combine_case(torch.bfloat16, count, dim, choices, 0.2, 62)
+    grad = _randn((count, dim), torch.bfloat16, 66)
+    for w in (weights, None):
+        want, _ = rows.combine_rows_grad(gpu_ctx, grad, data, position, w)
+        got = torch.zeros_like(data)
+        gpu_ctx.check(gpu_ctx.lib.glide_combine_rows_grad(gpu_ctx.handle, grad.data_ptr(), 3, count, dim, dim, data.data_ptr(), data.shape[0], dim, position.data_ptr(),
+                                                          choices, None if w is None else w.data_ptr(), got.data_ptr(), dim, None, torch.cuda.current_stream().cuda_stream))
+        assert torch.equal(got, want) and got.any()
+
+
+def test_dispatch_and_back_where_offsets_pass_32_bits(gpu_ctx):
+    count, dim, choices = 1_100_000, 2_048, 2      # 4.5e9 values sorted
+    data = torch.empty((count, dim), dtype=torch.float16, device="cuda")
+    data[:] = (torch.arange(count, device="cuda") % 2003 - 1001).half()[:, None]
+    data[:, 5] = (torch.arange(count, device="cuda") % 1999).half()
+    choice = _choice(count, choices, 3, 67)
+    d = rows.dispatch_rows(gpu_ctx, data, choice, 3)
+    _, which, start = _dispatch_want(choice, 3)
+    taken = int(start[-1])
+    assert taken * dim < 2 ** 32 < count * choices * dim
+    for a in list(range(0, taken, 200_000)):
+        assert torch.equal(d.d_sorted[a:min(a + 200_000, taken)], data[d.d_map[a:min(a + 200_000, taken)].long()])
+    assert np.array_equal(d.d_map.cpu().numpy(), which)
+    moved = torch.where(d.d_position >= 0, count * choices - 1 - d.d_position, -1)      # the same rows from the other end, beyond 2^32 values
+    flipped = d.d_sorted.flip(0)
+    times = (choice >= 0).sum(1, keepdim=True).half()
+    for position, held in ((d.d_position, d.d_sorted), (moved, flipped)):
+        back = rows.dispatch_rows_grad(gpu_ctx, held, position)
+        assert all(torch.equal(back[a:a + 100_000], data[a:a + 100_000] * times[a:a + 100_000]) for a in range(0, count, 100_000))
+    got, got_w = rows.combine_rows_grad(gpu_ctx, data, flipped, moved)
+    got = got.flip(0)
+    assert all(torch.equal(got[a:min(a + 200_000, taken)], d.d_sorted[a:min(a + 200_000, taken)]) for a in range(0, taken, 200_000))
+    assert not got[taken:].any()
+    size = torch.cat([(part.double() ** 2).sum(1) for part in data.split(100_000)])[:, None]
+    _close(got_w, torch.where(choice >= 0, size, 0.0), (dim + 2) * U * size)
 
 
 def test_combine_of_nothing(gpu_ctx):

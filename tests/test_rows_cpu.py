@@ -96,3 +96,17 @@ def test_workspaces_hold_what_the_calls_need():
     assert lib.glide_dispatch_rows_workspace(1 << 31, 1, 64) == 0
     assert lib.glide_lookup_rows_grad_workspace(1 << 32, 128, 10) == 0
     assert isinstance(C.c_size_t(lib.glide_lookup_rows_grad_workspace((1 << 32) - 1, 1 << 20, 0x7fffffff)).value, int)
+
+
+def test_the_workspace_of_a_gradient_holds_its_partial_sums():
+    """Two copies of the sorted ids with their rows, a rank of 2 bytes for each, a pass's counts for every 2,048 of them, and two rows of
+    fp32 sums for each chunk of at most 128; up to the largest call, whose need does not fit 32 bits by far."""
+    need = _lib.load().glide_lookup_rows_grad_workspace
+    for n in (1, 1000, 1 << 20, (1 << 32) - 1):
+        for dim in (1, 100, 4096, 1 << 20):
+            for count in (1025, 4097, 100_000, 0x7fffffff):
+                bits = max(1, (n).bit_length())                       # ids 0 .. n - 1, and n for none
+                passes = -(-bits // 11)
+                least = 18 * count + -(-count // 2048) * 4 * (1 << -(-bits // passes)) + 2 * -(-count // 128) * dim * 4
+                assert need(n, dim, count) >= least, (n, dim, count)
+                assert need(n, dim, count) <= 16 * least + (1 << 20)
