@@ -108,6 +108,8 @@ SIGNATURES = {
     "glide_dispatch_rows": (i32, [vp, vp, i32, u64, u32, u64, vp, u32, u32, vp, u64, vp, vp, vp, vp, C.c_size_t, vp]),
     "glide_combine_rows": (i32, [vp, vp, i32, u64, u32, u64, vp, u64, u32, vp, vp, u64, vp]),
     "glide_combine_rows_grad": (i32, [vp, vp, i32, u64, u32, u64, vp, u64, u64, vp, u32, vp, vp, u64, vp, vp]),
+    "glide_clear_rows_without_place_workspace": (C.c_size_t, [u64]),
+    "glide_clear_rows_without_place": (i32, [vp, vp, i32, u64, u32, u64, vp, u64, vp, C.c_size_t, vp]),
     "glide_malloc": (i32, [vp, C.c_size_t, P(vp)]),
     "glide_memcpy_h2d": (i32, [vp, vp, vp, C.c_size_t]),
     "glide_memcpy_d2h": (i32, [vp, vp, vp, C.c_size_t]),

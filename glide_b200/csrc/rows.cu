@@ -676,17 +676,17 @@ __device__ __forceinline__ void name_rows(const GradArgs &a, uint32_t r0, uint32
 
 // Rows [r0, r1) that `mark` does not name are cleared.
 template<typename O, typename Mark>
-__device__ __forceinline__ void clear_rows(const Rows<O> &out, const GradArgs &a, uint32_t r0, uint32_t r1, Mark mark) {
+__device__ __forceinline__ void clear_rows(const Rows<O> &out, uint32_t dim, const Div &by_row_bytes, uint32_t r0, uint32_t r1, Mark mark) {
     __shared__ uint32_t named[256 / 32];
     if (threadIdx.x < 8) named[threadIdx.x] = 0;
     __syncthreads();
     mark(named);
     __syncthreads();
     uint8_t *at = reinterpret_cast<uint8_t *>(out.row(r0));
-    const uint64_t row_bytes = (uint64_t) a.dim * sizeof(O);
-    if (out.stride == a.dim && row_bytes >= 16) {   // a word of 16 bytes lies in two rows at most; one that lies in a named and another one goes out in halves
+    const uint64_t row_bytes = (uint64_t) dim * sizeof(O);
+    if (out.stride == dim && row_bytes >= 16) {   // a word of 16 bytes lies in two rows at most; one that lies in a named and another one goes out in halves
         const auto is_named = [&](uint32_t byte) {
-            const uint32_t r = a.by_row_bytes.of(byte);
+            const uint32_t r = by_row_bytes.of(byte);
             return (named[r >> 5] >> (r & 31u) & 1u) != 0;
         };
         clear_bytes(at, 0, (r1 - r0) * row_bytes, [&](uint32_t first, uint32_t last) {
@@ -700,9 +700,9 @@ __device__ __forceinline__ void clear_rows(const Rows<O> &out, const GradArgs &a
         for (uint32_t r = 0; r < r1 - r0; r++)
             if (!(named[r >> 5] >> (r & 31u) & 1u)) clear_bytes(at + r * out.stride * sizeof(O), 0, row_bytes, [](uint32_t, uint32_t) { return false; });
     } else {
-        for (uint32_t x = threadIdx.x; x < (r1 - r0) * a.dim; x += blockDim.x) {
-            const uint32_t r = x / a.dim;
-            if (!(named[r >> 5] >> (r & 31u) & 1u)) out.row(r0 + r)[x - r * a.dim] = from_float<O>(0.0f);
+        for (uint32_t x = threadIdx.x; x < (r1 - r0) * dim; x += blockDim.x) {
+            const uint32_t r = x / dim;
+            if (!(named[r >> 5] >> (r & 31u) & 1u)) out.row(r0 + r)[x - r * dim] = from_float<O>(0.0f);
         }
     }
 }
@@ -719,7 +719,7 @@ __global__ void __launch_bounds__(256, 4) grad_join_kernel(Rows<const T> grad, R
     if (blockIdx.x >= a.join_blocks) {
         const uint64_t r0 = a.clear_from + (uint64_t) (blockIdx.x - a.join_blocks) * a.clear_rows;
         const uint32_t r1 = (uint32_t) min((uint64_t) a.n, r0 + a.clear_rows);
-        return clear_rows(out, a, (uint32_t) r0, r1, [&](uint32_t *named) { name_rows(a, (uint32_t) r0, r1, named); });
+        return clear_rows(out, a.dim, a.by_row_bytes, (uint32_t) r0, r1, [&](uint32_t *named) { name_rows(a, (uint32_t) r0, r1, named); });
     }
     const uint32_t group = (blockIdx.x * 256 + threadIdx.x) / a.lanes, lane = threadIdx.x & (a.lanes - 1);
     const uint32_t chunk = group / a.slabs, word = (group - chunk * a.slabs) * a.lanes + lane;
@@ -784,7 +784,7 @@ __global__ void __launch_bounds__(256) grad_few_kernel(Rows<const T> grad, Rows<
     if (blockIdx.x >= a.items) {
         const uint64_t r0 = (uint64_t) (blockIdx.x - a.items) * a.clear_rows;
         const uint32_t r1 = (uint32_t) min((uint64_t) a.n, r0 + a.clear_rows);
-        return clear_rows(out, a, (uint32_t) r0, r1, [&](uint32_t *named) {
+        return clear_rows(out, a.dim, a.by_row_bytes, (uint32_t) r0, r1, [&](uint32_t *named) {
             for (uint32_t i = threadIdx.x; i < a.items; i += 256)
                 if (keys[i] >= r0 && keys[i] < r1) atomicOr(&named[(keys[i] - (uint32_t) r0) >> 5], 1u << ((keys[i] - (uint32_t) r0) & 31u));
         });
@@ -1208,6 +1208,27 @@ __global__ void __launch_bounds__(256) combine_grad_kernel(Rows<const T> grad, u
             __syncthreads();
         }
     }
+}
+
+// ---- rows without a place -------------------------------------------------------------------------------------------
+// A bit for each row that a position names, then a CTA looks at the bits of `each` rows (32 to 256, some 128 KB) and clears those without one. Rows
+// that are named cost a bit each: 131,072 rows of 4 KB, 2 % of them without a place, take 15 us, as zeros for all of them before take 140.
+__global__ void __launch_bounds__(256) mark_places_kernel(const uint32_t *__restrict__ position, uint32_t pairs, uint32_t rows, uint32_t *marks) {
+    const uint32_t i = blockIdx.x * 256 + threadIdx.x;
+    const uint32_t p = i < pairs ? position[i] : kNone;
+    if (p < rows) atomicOr(marks + (p >> 5), 1u << (p & 31u));
+    let_next_start();
+}
+template<typename O>
+__global__ void __launch_bounds__(256) clear_unplaced_kernel(Rows<O> out, uint32_t rows, uint32_t dim, Div by_row_bytes, uint32_t each, const uint32_t *marks) {
+    wait_for_previous();
+    const uint32_t r0 = blockIdx.x * each, r1 = r0 + min(each, rows - r0), words = (r1 - r0 + 31) / 32;
+    const uint32_t mine = threadIdx.x < words ? __ldcg(marks + r0 / 32 + threadIdx.x) : 0xffffffffu;
+    const uint32_t there = threadIdx.x + 1 == words && (r1 & 31u) ? (1u << (r1 & 31u)) - 1 : 0xffffffffu;   // bits of rows that there are
+    if (__syncthreads_and((mine & there) == there)) return;
+    clear_rows(out, dim, by_row_bytes, r0, r1, [&](uint32_t *named) {
+        if (threadIdx.x < words) named[threadIdx.x] = mine;
+    });
 }
 
 // ---- host side ----------------------------------------------------------------------------------------------------
@@ -1684,6 +1705,41 @@ int glide_combine_rows_grad(glide_ctx *ctx, const void *d_grad, int row_type, ui
         // eight lanes a row of up to 32 pieces: 92,324 x 3 rows of 64 bytes 33 against 15 us, 100,000 x 2 of 512 bytes 50 against 43
         return words <= 32 ? lanes(Number<8>{}) : lanes(Number<32>{});
     }));
+    return GLIDE_OK;
+}
+
+size_t glide_clear_rows_without_place_workspace(uint64_t rows) { return rows > 0x7fffffffu ? 0 : (size_t) align256(ceil_div(rows, 32) * 4); }
+
+int glide_clear_rows_without_place(glide_ctx *ctx, void *d_rows, int row_type, uint64_t rows, uint32_t dim, uint64_t row_stride, const uint32_t *d_position,
+                                   uint64_t pairs, void *d_workspace, size_t workspace_bytes, void *stream) {
+    ROWS_REQUIRE(ctx, GLIDE_ERR_BAD_ARG, "clear_rows_without_place: null context");
+    ROWS_REQUIRE(is_float_type(row_type), GLIDE_ERR_UNSUPPORTED, "clear_rows_without_place: unsupported row type %d", row_type);
+    ROWS_REQUIRE(dim >= 1, GLIDE_ERR_BAD_ARG, "clear_rows_without_place: no values");
+    ROWS_REQUIRE(dim <= kMaxDim && rows <= 0x7fffffffu && pairs <= 0x7fffffffu, GLIDE_ERR_UNSUPPORTED, "clear_rows_without_place: more than 2^20 values or 2^31 - 1 pairs or rows");
+    if (rows == 0) return GLIDE_OK;
+    const Matrix out{d_rows, rows, row_stride, dim, row_type};
+    ROWS_REQUIRE(d_rows && (d_position || pairs == 0), GLIDE_ERR_BAD_ARG, "clear_rows_without_place: null pointer");
+    ROWS_REQUIRE(out.sized() && (row_stride >= dim || rows == 1), GLIDE_ERR_BAD_ARG, "clear_rows_without_place: rows overlap, or are beyond 2^60 values");
+    ROWS_REQUIRE(aligned(out) && reinterpret_cast<uintptr_t>(d_position) % 4 == 0, GLIDE_ERR_BAD_ARG, "clear_rows_without_place: a pointer is not aligned to its type");
+    const size_t need = glide_clear_rows_without_place_workspace(rows);
+    ROWS_REQUIRE(workspace_bytes >= need && d_workspace, GLIDE_ERR_BAD_ARG, "clear_rows_without_place: the workspace has %zu bytes, %zu are needed", workspace_bytes, need);
+    ROWS_REQUIRE(reinterpret_cast<uintptr_t>(d_workspace) % 256 == 0, GLIDE_ERR_BAD_ARG, "clear_rows_without_place: the workspace is not aligned to 256 bytes");
+    ROWS_REQUIRE(!overlap(d_rows, out.bytes(), d_position, pairs * 4) && !overlap(d_workspace, need, d_rows, out.bytes()) && !overlap(d_workspace, need, d_position, pairs * 4),
+                 GLIDE_ERR_BAD_ARG, "clear_rows_without_place: the rows or the workspace overlap another argument");
+    const OnDevice guard(ctx->device);
+    ROWS_CUDA(guard.status);
+    auto s = static_cast<cudaStream_t>(stream);
+    uint32_t *marks = static_cast<uint32_t *>(d_workspace);
+    ROWS_CUDA(cudaMemsetAsync(marks, 0, ceil_div(rows, 32) * 4, s));
+    if (pairs) ROWS_CUDA(launch(mark_places_kernel, ceil_div(pairs, 256), 256, 0, s, false, d_position, (uint32_t) pairs, (uint32_t) rows, marks));
+    const uint32_t row_bytes = dim * bytes_of(row_type);
+    uint32_t each = (128u << 10) / row_bytes / 32 * 32;
+    each = each < 32 ? 32 : each > 256 ? 256 : each;
+    auto clear = [&](auto o) {   // zeros have the same bits in both types of 16 bits
+        using O = decltype(o);
+        return launch(clear_unplaced_kernel<O>, ceil_div(rows, each), 256, 0, s, pairs != 0, out.as<O>(), (uint32_t) rows, dim, Div(row_bytes), each, marks);
+    };
+    ROWS_CUDA(bytes_of(row_type) == 4 ? clear(float{}) : clear(__half{}));
     return GLIDE_OK;
 }
 

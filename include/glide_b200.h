@@ -451,6 +451,11 @@ int glide_combine_rows_grad(glide_ctx *ctx, const void *d_grad, int row_type, ui
                             const void *d_sorted, uint64_t sorted_rows, uint64_t sorted_stride, const uint32_t *d_position,
                             uint32_t choices, const float *d_weights_or_null, void *d_grad_sorted, uint64_t grad_sorted_stride,
                             float *d_grad_weights_or_null, void *stream);
+/* Zeros for the rows that none of the positions names; the others are not touched. For a d_grad_sorted (or d_sorted) that is not
+ * clear, where some choices may be missing and all rows are read: it costs less than clearing every row before. */
+size_t glide_clear_rows_without_place_workspace(uint64_t rows);
+int glide_clear_rows_without_place(glide_ctx *ctx, void *d_rows, int row_type, uint64_t rows, uint32_t dim, uint64_t row_stride,
+                                   const uint32_t *d_position, uint64_t pairs, void *d_workspace, size_t workspace_bytes, void *stream);
 
 /* ---- device memory helpers for hosts without their own CUDA binding --------------------- */
 int glide_malloc(glide_ctx *ctx, size_t bytes, void **d_out);

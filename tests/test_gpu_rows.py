@@ -546,6 +546,77 @@ def test_combine_grad_makes_zeros_of_rows_without_a_place(gpu_ctx, dtype, count,
         assert (got[rest] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("count,dim,choices,empty", [(16_000, 600, 4, 0.02), (9001, 1001, 8, 0.6), (50_000, 520, 2, 0.0), (70_000, 520, 1, 1.0)])
+def test_combine_grad_makes_zeros_in_large_results(gpu_ctx, dtype, count, dim, choices, empty):
+    """More bytes than are cleared whole, places in any order, memory that held NaN: as with a result of zeros that is handed in."""
+    data, position, weights = _combine_case(dtype, count, dim, choices, empty, 68)
+    place = torch.randperm(count * choices, generator=_gen(71), device="cuda").int()
+    position = torch.where(position >= 0, place[position.clamp(min=0).long()], -1).contiguous()
+    grad = _randn((count, dim), dtype, 72)
+    assert data.numel() * data.element_size() > rows._FEW_BYTES
+    want, want_w = rows.combine_rows_grad(gpu_ctx, grad, data, position, weights, out=torch.zeros_like(data))
+    torch.full(data.shape, float("nan"), dtype=dtype, device="cuda")
+    got, got_w = rows.combine_rows_grad(gpu_ctx, grad, data, position, weights)
+    assert torch.equal(got, want) and torch.equal(got_w, want_w)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,stride,offset", [(1, 1, 1), (1, 3, 0), (5, 5, 1), (7, 8, 0), (8, 8, 0), (20, 33, 1), (100, 100, 3), (136, 136, 1), (264, 271, 0), (40_000, 40_001, 1), (70_000, 70_000, 0)])
+def test_rows_without_a_place_are_cleared_and_nothing_else(gpu_ctx, dtype, dim, stride, offset):
+    """None, some and all of the rows with a place, positions beyond the rows, the same position twice; in captured calls, too."""
+    lib, stream = gpu_ctx.lib, torch.cuda.current_stream().cuda_stream
+    for n in (1, 31, 32, 33, 255, 256, 257, 1000):
+        if n * dim > 20_000_000:
+            continue
+        scratch = torch.full((lib.glide_clear_rows_without_place_workspace(n),), 255, dtype=torch.uint8, device="cuda")
+        for share in (0.0, 0.4, 0.97, 1.0):
+            named = torch.rand((n,), generator=_gen(170 + n), device="cuda") < share
+            at = torch.nonzero(named).reshape(-1).int()
+            position = torch.cat([at, torch.tensor([-1, n, 2 ** 31 - 1], dtype=torch.int32, device="cuda"), at[:3]])[torch.randperm(at.numel() + 3 + at[:3].numel(), device="cuda")]
+            held, whole = _strided((n, dim), dtype, 171, stride, offset)
+            whole.fill_(float("nan"))
+            gpu_ctx.check(lib.glide_clear_rows_without_place(gpu_ctx.handle, held.data_ptr(), rows._FLOATS[dtype], n, dim, stride, position.data_ptr(), position.numel(),
+                                                             scratch.data_ptr(), scratch.numel(), stream))
+            assert held[named].isnan().all() and (held[~named] == 0).all()
+            mask = torch.zeros_like(whole, dtype=torch.bool)
+            mask.as_strided((n, dim), (stride, 1), offset).fill_(True)
+            assert whole[~mask].isnan().all()
+    held = torch.ones((4, dim), dtype=dtype, device="cuda")
+    gpu_ctx.check(lib.glide_clear_rows_without_place(gpu_ctx.handle, held.data_ptr(), rows._FLOATS[dtype], 4, dim, dim, None, 0, scratch.data_ptr(), scratch.numel(), stream))
+    assert not held.any()
+
+
+def test_clearing_rows_without_a_place_is_captured_and_its_refusals(gpu_ctx):
+    lib, h = gpu_ctx.lib, gpu_ctx.handle
+    held, position = torch.ones((5000, 40), device="cuda"), torch.arange(0, 5000, 2, dtype=torch.int32, device="cuda")
+    scratch = torch.full((lib.glide_clear_rows_without_place_workspace(5000),), 255, dtype=torch.uint8, device="cuda")
+    H, P, W, S = held.data_ptr(), position.data_ptr(), scratch.data_ptr(), scratch.numel()
+    g = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        gpu_ctx.check(lib.glide_clear_rows_without_place(h, H, 0, 5000, 40, 40, P, 2500, W, S, torch.cuda.current_stream().cuda_stream))
+    for shift in (0, 1):
+        held.fill_(1)
+        position.copy_(torch.arange(shift, 5000, 2, dtype=torch.int32, device="cuda"))
+        g.replay()
+        assert (held[shift::2] == 1).all() and (held[1 - shift::2] == 0).all()
+    del g
+    held.fill_(1)
+
+    def clear(code, r=H, kind=0, n=5000, dim=40, stride=40, p=P, pairs=2500, w=W, wb=S):
+        assert lib.glide_clear_rows_without_place(h, r, kind, n, dim, stride, p, pairs, w, wb, None) == code
+        assert code == 0 or len(lib.glide_last_error(h)) > 10
+
+    clear(0, n=0)
+    for wrong in (dict(r=None), dict(p=None), dict(w=None), dict(wb=S - 1), dict(dim=0), dict(stride=39), dict(r=H + 2), dict(p=P + 1), dict(w=W + 16), dict(p=H), dict(w=H), dict(stride=1 << 60)):
+        clear(-1, **wrong)
+    for wrong in (dict(kind=1), dict(kind=4), dict(dim=1 << 21), dict(n=1 << 31), dict(pairs=1 << 31)):
+        clear(-2, **wrong)
+    torch.cuda.synchronize()
+    assert (held == 1).all()
+
+
 def test_combine_leaves_out_what_has_no_place_whatever_it_would_hold(gpu_ctx):
     data = _randn((6, 40), torch.float32, 50)
     data[5] = float("nan")

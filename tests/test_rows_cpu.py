@@ -110,3 +110,11 @@ def test_the_workspace_of_a_gradient_holds_its_partial_sums():
                 least = 18 * count + -(-count // 2048) * 4 * (1 << -(-bits // passes)) + 2 * -(-count // 128) * dim * 4
                 assert need(n, dim, count) >= least, (n, dim, count)
                 assert need(n, dim, count) <= 16 * least + (1 << 20)
+
+
+def test_the_workspace_for_rows_without_a_place_has_a_bit_for_each():
+    lib = _lib.load()
+    for n in (0, 1, 32, 33, 1 << 20, 0x7fffffff):
+        assert n / 8 <= lib.glide_clear_rows_without_place_workspace(n) <= n / 8 + 512
+    assert lib.glide_clear_rows_without_place_workspace(1 << 31) == 0
+    assert lib.glide_clear_rows_without_place(None, None, 0, 1, 1, 1, None, 0, None, 0, None) == -1
