@@ -29,7 +29,9 @@ constexpr uint32_t kRounds = 8;             // items of a thread in the counting
 constexpr uint32_t kTileThreads = 256, kTile = kTileThreads * kRounds;
 constexpr uint32_t kFew = 4096;             // items that are sorted by comparing each with all (the gradient of 4,000 ids of 64 bf16: 15 us, of 4,097 in tiles: 20)
 constexpr uint32_t kFewPairs = 2048;        // pairs that dispatch_rows places and copies in one launch (2,000: 6 to 8 us, in tiles 8; 4,000: 14 to 19, in tiles 8 to 10)
-constexpr uint32_t kFewIds = 1024;          // ids whose gradient takes one launch (see grad_few_kernel)
+// Ids whose gradient takes one launch (see grad_few_kernel), whatever they are: 1,024 different ones, added to a table of 64, 512 and 4,096 bf16 a row, 7,
+// 8 and 10 us, by the sort 10, 10 and 11. The other side: one CTA adds up an id, so that 1,024 equal ones take 7, 27 and 187 us, by the sort 13, 14 and 15.
+constexpr uint32_t kFewIds = 1024;
 constexpr uint32_t kMaxPassBits = 11;       // bits of a pass's digit, at most
 constexpr uint32_t kMaxFusedCounts = 16384; // counts (tiles x buckets) that every CTA of the second kernel adds up by itself (64 x 1,001 of them: 19.5 us, scanned by a launch of their own 13.9)
 constexpr uint32_t kClearShare = 48u << 20; // bytes of a gradient that are cleared beside each launch of its sort (12 to 64 MB differ by 3 %)
@@ -198,7 +200,7 @@ struct Div {
 // ---- lookup -------------------------------------------------------------------------------------------------
 // out[t] = scale * table[ids[t]], zeros for ids beyond the table (0xffffffff among them). A thread owns U pieces of the output, a
 // CTA's width apart, so that U loads are in flight once the ids (which a CTA shares through L1) have come: 2 for large calls (1 takes a
-// quarter longer, 4 as long), 1 where 2 would leave SMs idle. 32,768 ids over 131,072 rows of 8 KB: 64 us, 88 % of the copy rate; bound by
+// quarter longer, 4 as long), 1 where 2 would leave SMs idle. 32,768 ids over 131,072 rows of 8 KB: 64 us, 87 % of the copy rate; bound by
 // DRAM and, a little, by the wait for the ids.
 template<typename T, typename O, int V, bool kWhole, int U>
 __global__ void __launch_bounds__(256) lookup_kernel(Rows<const T> table, uint32_t n, uint32_t dim, const uint32_t *__restrict__ ids, uint32_t units, Div words,
@@ -290,7 +292,7 @@ cudaError_t launch(void (*kernel)(P...), uint64_t grid, uint32_t block, uint32_t
 // One pass places every item behind all items of a smaller digit and behind the items of its own digit that came before it.
 // A CTA takes a tile of consecutive items, each of its warps a run of 256, 32 at a time: a lane's rank among the items of
 // its digit is the warp's running count plus the equal digits at lower lanes, and a scan over the warps' counts makes it the
-// rank in the tile. No atomics: the order depends on nothing but the keys. Few launches count most here (the data are 6 to 10
+// rank in the tile. The order depends on nothing but the keys (atomics only add up counts, in shared memory). Few launches count most here (the data are 6 to 10
 // bytes an item): up to kFew items are sorted by one launch that compares each with all, more by two launches a pass while every CTA
 // of the second can add up the counts of all tiles, else by three. A launch takes 2 to 4 us of latency, whatever its size. Tiles are
 // small because their items' scattered stores leave an SM at one sector a cycle: in tiles of 8,192 a pass over 100,000 ids took 31 us,
@@ -710,8 +712,8 @@ __device__ __forceinline__ void clear_rows(const Rows<O> &out, uint32_t dim, con
 // A group of lanes joins a chunk of sorted items over a slab of the row: the sum of a run of equal ids goes to the id's row, or,
 // where the run goes on in another chunk, to the chunk's partial sums (first: it came from the chunk before). Consecutive items of a
 // sorted list make equal shares of any distribution of ids, be it one id. The other CTAs clear the rows that no id names.
-// 32,768 tokens over 131,072 rows of 8 KB (1.3 GB with the cleared rows): 222 us with its sort, 93 % of the copy rate; 100,000 ids over a
-// million rows of 512 bytes: 103 us, 84 %, of which the sort's latency is the rest.
+// 32,768 tokens over 131,072 rows of 8 KB (1.3 GB with the cleared rows): 221 us with its sort, 93 % of the copy rate; 100,000 ids over a
+// million rows of 512 bytes: 105 us, 82 %, of which the sort's latency is the rest.
 template<typename T, typename O, int V>
 __global__ void __launch_bounds__(256, 4) grad_join_kernel(Rows<const T> grad, Rows<O> out, GradArgs a) {
     constexpr int U = in_flight(64, V * (int) sizeof(T), 8);
@@ -1043,7 +1045,7 @@ __global__ void __launch_bounds__(256) dispatch_small_kernel(Rows<const T> rows,
 
 // ---- combine ----------------------------------------------------------------------------------------------------
 // out[t] = sum over j, ascending, of weight[t,j] * sorted[position[t,j]]; K pairs' pieces are in flight for each piece of a row: as many
-// as there are choices, up to 8. 16,384 x 8 rows of 4 KB: 92 us, 98 % of the copy rate.
+// as there are choices, up to 8. 16,384 x 8 rows of 4 KB: 96 us, 94 % of the copy rate.
 template<typename T, int V, bool kWhole, int K>
 __global__ void __launch_bounds__(256) combine_kernel(Rows<const T> sorted, uint32_t sorted_rows, uint32_t dim, const uint32_t *__restrict__ position,
                                                       uint32_t choices, const float *__restrict__ weights, uint32_t units, Div words, Rows<T> out) {
